@@ -45,7 +45,7 @@ extern "C" {
 #define NSB_API
 #endif
 
-#define NSB_ABI_VERSION 14
+#define NSB_ABI_VERSION 15
 
 enum nsb_status {
   NSB_OK = 0,
@@ -544,6 +544,105 @@ NSB_API int nsb_dendritic_event_hybrid(const nsb_tick* tick, float* current,
                                        uint64_t gate_edges, const nsb_tick_out* out,
                                        const nsb_out* out_emitted, void* workspace,
                                        size_t workspace_bytes, int* status, void* stream);
+
+/* -------------------------------------------------------------------------
+ * Token operators: the two ends of a token model around the simulated network
+ * (token -> drive -> ticks -> state -> logits -> token).  No counterpart in the
+ * reference's extension.  Values are float32, float16 or bfloat16; every sum,
+ * norm and scale is float32.  A call with no rows does nothing.
+ * ------------------------------------------------------------------------- */
+enum nsb_value_type { NSB_VALUE_F32 = 0, NSB_VALUE_F16 = 1, NSB_VALUE_BF16 = 2 };
+
+/* A matrix with contiguous rows: element (r, c) at data[r * row_stride + c]. */
+typedef struct nsb_matrix {
+  void* data;
+  int64_t rows, cols;
+  int64_t row_stride; /* elements, >= cols */
+  int32_t type;       /* enum nsb_value_type */
+} nsb_matrix;
+
+/* out[t, :] = scale * table[tokens[t], :], rounded once; a zero row where a token lies
+ * outside [0, table->rows).  `tokens`: out->rows int32 or int64 (`token_bytes` 4 or 8).
+ * `out` has the table's type or float32.  One launch. */
+NSB_API int nsb_stimulus_drive(const void* tokens, int32_t token_bytes, const nsb_matrix* table,
+                               float scale, const nsb_matrix* out, void* stream);
+
+/* The gradient of the table: out[v, :] = scale * (sum of grad[t, :] over tokens[t] = v), all rows
+ * written, summed in float32 in an order that the tokens alone fix (deterministic).  Where the
+ * types of `grad` and `out` differ, one of them is float32.  Workspace: 16-byte aligned, contents need not be initialised. */
+NSB_API size_t nsb_stimulus_gradient_workspace_size(int64_t tokens, int64_t cols);
+NSB_API int nsb_stimulus_gradient(const void* tokens, int32_t token_bytes, const nsb_matrix* grad,
+                                  float scale, const nsb_matrix* out, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+
+/* A dense NVFP4 matrix.  Row r's scale g = max(amax / 2688, FLT_MIN) over the row (scale_count =
+ * rows) or the whole matrix (scale_count = 1); per 16 consecutive columns an E4M3 block scale
+ * s = e4m3(min(block_amax / (6 g), 448)) and E2M1 codes of |x| / (g s) (ties to the even code, the
+ * sign in bit 3): value = level * (s g).  With one scale this is nsb_encode_weights' format, row by row.
+ *   codes         [rows, code_stride]: two per byte, the even column in the low nibble;
+ *                 code_stride = 16 * ceil(cols / 32) bytes; 16-byte aligned
+ *   block_scales  [ceil(rows / 128), 4 * ceil(cols / 256), 512]: tile (i, j) holds rows 128 i ... and
+ *                 blocks 4 j ..., row r's block b at byte 16 (r % 32) + 4 (r % 128 / 32) + b % 4; 16-byte aligned
+ * Codes and block scales beyond `cols` are zero.  A row (matrix) with an infinity or a NaN gets the
+ * scale NaN and zero codes. */
+typedef struct nsb_nvfp4 {
+  int64_t rows, cols;
+  uint8_t* codes;
+  int64_t code_stride;
+  uint8_t* block_scales;
+  float* scale;
+  int64_t scale_count; /* rows or 1 */
+} nsb_nvfp4;
+
+/* `out` = the NVFP4 form of `value` (transpose = 0: out->rows = value->rows) or of its transpose.
+ * Workspace: 4-byte aligned, contents need not be initialised (may be NULL where the size is 0). */
+NSB_API size_t nsb_nvfp4_quantize_workspace_size(int64_t rows, int64_t cols, int32_t transpose,
+                                                 int64_t scale_count);
+NSB_API int nsb_nvfp4_quantize(const nsb_matrix* value, int32_t transpose, const nsb_nvfp4* out,
+                               void* workspace, size_t workspace_bytes, void* stream);
+NSB_API int nsb_nvfp4_dequantize(const nsb_nvfp4* value, const nsb_matrix* out, void* stream);
+
+/* out[m, n] = sum over k of a[m, k] b[n, k], plus bias[n] where bias is given (float32).  Sums are
+ * float32; the result depends on the operands only (deterministic).  Bounded waits inside the kernel
+ * write a code other than 0 to *status (device, may be NULL) where they give up. */
+NSB_API int nsb_nvfp4_product(const nsb_nvfp4* a, const nsb_nvfp4* b, const float* bias,
+                              const nsb_matrix* out, int* status, void* stream);
+
+/* out[c] = sum of column c of `value` (float32, in a fixed order): the gradient of a bias. */
+NSB_API size_t nsb_column_sums_workspace_size(int64_t rows, int64_t cols);
+NSB_API int nsb_column_sums(const nsb_matrix* value, float* out, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/* One float32 per row: data[r * stride], or `scalar` where data is NULL. */
+typedef struct nsb_row_values {
+  const float* data;
+  int64_t stride;
+  float scalar;
+} nsb_row_values;
+
+/* Logits after penalties, biases and masks, and the greedy choice.  For token v of row b, with c its
+ * occurrences among history[b, prompt_lengths[b] .. lengths[b]) and `seen` whether it occurs in
+ * history[b, 0 .. lengths[b]) at all:
+ *   x = logits[b, v];   if seen: x = x > 0 ? x / repetition : x * repetition
+ *   x = x - frequency * c;   if c > 0: x = x - presence;   x = x + bias[v]
+ *   out[b, v] = mask bit v of the row ? x : -inf      (bit v % 32 of word v / 32)
+ * in float32, each step rounded, the result rounded to out's type.  choice[b] is the lowest index
+ * of the row's largest out value, -1 where none is above -inf (NaN is never chosen).  Lengths are
+ * clamped to [0, history_length]; history entries outside [0, vocabulary) are skipped. */
+typedef struct nsb_logits {
+  nsb_matrix logits, out;  /* [rows, vocabulary], same type; out may be the logits themselves */
+  const int32_t* history;  /* [rows, history_length] */
+  int64_t history_length, history_stride;
+  const int32_t* lengths;        /* [rows], NULL: history_length */
+  const int32_t* prompt_lengths; /* [rows], NULL: 0 */
+  nsb_row_values repetition, presence, frequency; /* neutral: 1, 0, 0 */
+  const float* bias;       /* NULL: none */
+  int64_t bias_stride;     /* elements between rows, 0: one bias for all rows */
+  const int32_t* mask;     /* NULL: all allowed */
+  int64_t mask_stride;     /* words between rows, 0: one mask for all rows */
+  int64_t* choice;         /* [rows], NULL: not wanted */
+} nsb_logits;
+NSB_API int nsb_adjust_logits(const nsb_logits* args, void* stream);
 
 /* NSB_ABI_VERSION of the loaded library. */
 NSB_API int nsb_abi_version(void);

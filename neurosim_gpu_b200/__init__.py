@@ -6,15 +6,20 @@ layout, with every inference tick running in ``libneurosim_b200.so``.
 """
 
 from .dynamics import DendriticDynamics, Dynamics
+from .logits import adjust_logits
+from .microscale import (Nvfp4Matrix, check_product_status, nvfp4_product, nvfp4_readout,
+                         quantize_nvfp4)
 from .native import load_native_extension
 from .precision import PRECISIONS, encode_sparse_weights, quantize_dequantize
 from .runtime import (NativeDendriticMatrixRuntime, NativeDendriticPELSRuntime, RuntimeStats,
                       validate_emission_threshold)
+from .stimulus import stimulus_drive, stimulus_gradient
 from .topology import SparseTopology, random_topology
 
 __all__ = [
     "DendriticDynamics", "Dynamics", "NativeDendriticMatrixRuntime",
-    "NativeDendriticPELSRuntime", "PRECISIONS", "RuntimeStats", "SparseTopology",
-    "encode_sparse_weights", "load_native_extension", "quantize_dequantize",
-    "random_topology", "validate_emission_threshold",
+    "NativeDendriticPELSRuntime", "Nvfp4Matrix", "PRECISIONS", "RuntimeStats", "SparseTopology",
+    "adjust_logits", "check_product_status", "encode_sparse_weights", "load_native_extension",
+    "nvfp4_product", "nvfp4_readout", "quantize_dequantize", "quantize_nvfp4",
+    "random_topology", "stimulus_drive", "stimulus_gradient", "validate_emission_threshold",
 ]

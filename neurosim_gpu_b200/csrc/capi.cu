@@ -10,6 +10,7 @@
 #include <string>
 
 #include "nsb_launch.h"
+#include "nsb_tokens.h"
 
 namespace nsb {
 size_t event_workspace_bytes(int64_t batch, int64_t neurons);
@@ -103,6 +104,27 @@ bool check_width(int32_t width) {
 }
 
 }  // namespace
+
+namespace nsb {
+
+int set_error(int code, const char* message) noexcept {
+  try {
+    g_error = message;
+  } catch (...) {  // no memory for the message: the code alone
+    g_error.clear();
+  }
+  return code;
+}
+
+int set_cuda_error(cudaError_t err, const char* where) noexcept {
+  try {
+    return cuda_fail(err, where);
+  } catch (...) {
+    return set_error(NSB_ERR_CUDA, "");
+  }
+}
+
+}  // namespace nsb
 
 extern "C" {
 

@@ -1,0 +1,199 @@
+// capi_tokens.cu -- extern "C" entry points of the token operators (see include/neurosim_b200.h).
+//
+// As in capi.cu, arguments are checked completely before anything is enqueued; a failed check
+// returns a negative status and leaves a message for nsb_last_error().  Nothing here throws.
+#include "nsb_tokens.h"
+
+namespace {
+
+constexpr int64_t kMost = int64_t{1} << 31;  // rows, columns and tokens are below this
+
+bool fail(const char* message) { return nsb::set_error(NSB_ERR_ARGUMENT, message), false; }
+
+bool type_ok(int32_t type) {
+  return type == NSB_VALUE_F32 || type == NSB_VALUE_F16 || type == NSB_VALUE_BF16;
+}
+
+bool check_matrix(const nsb_matrix* m, nsb::Dense* d, const char* shape, const char* data) {
+  if (!m || m->rows < 0 || m->cols < 1 || m->rows >= kMost || m->cols >= kMost || m->row_stride < m->cols ||
+      !type_ok(m->type))
+    return fail(shape);
+  if (m->rows > 0 && (!m->data || reinterpret_cast<uintptr_t>(m->data) % nsb::value_bytes(m->type) != 0))
+    return fail(data);
+  *d = {m->data, m->rows, m->cols, m->row_stride, m->type};
+  return true;
+}
+
+bool check_tokens(const void* tokens, int32_t bytes, int64_t n) {
+  if (bytes != 4 && bytes != 8) return fail("tokens must be int32 or int64");
+  if (n > 0 && (!tokens || reinterpret_cast<uintptr_t>(tokens) % bytes != 0)) return fail("tokens are required, aligned to their size");
+  return true;
+}
+
+bool check_nvfp4(const nsb_nvfp4* m, nsb::Nvfp4* d) {
+  if (!m || m->rows < 0 || m->cols < 1 || m->rows >= kMost || m->cols >= kMost)
+    return fail("an NVFP4 matrix is [rows >= 0, cols >= 1], each below 2^31");
+  if (m->code_stride != (m->cols + 31) / 32 * 16) return fail("NVFP4 codes: rows must be 16 * ceil(cols / 32) bytes apart");
+  if (m->scale_count != m->rows && m->scale_count != 1) return fail("NVFP4 scale: one value per row, or one");
+  if (m->rows > 0 && (!m->codes || !m->block_scales || !m->scale)) return fail("NVFP4 codes, block scales and scale are required");
+  if (reinterpret_cast<uintptr_t>(m->codes) % 16 != 0 || reinterpret_cast<uintptr_t>(m->block_scales) % 16 != 0 ||
+      reinterpret_cast<uintptr_t>(m->scale) % 4 != 0)
+    return fail("NVFP4 codes and block scales must be 16-byte aligned, the scale 4-byte aligned");
+  *d = {m->rows, m->cols, m->codes, m->code_stride, m->block_scales, m->scale, m->scale_count != 1};
+  return true;
+}
+
+bool check_workspace(const void* workspace, size_t have, size_t need, size_t align) {
+  if (need == 0) return true;
+  if (workspace && have >= need && reinterpret_cast<uintptr_t>(workspace) % align == 0) return true;
+  nsb::set_error(NSB_ERR_WORKSPACE, "workspace missing, misaligned or too small");
+  return false;
+}
+
+int done(cudaError_t err, const char* where) {
+  return err == cudaSuccess ? NSB_OK : nsb::set_cuda_error(err, where);
+}
+
+}  // namespace
+
+extern "C" {
+
+int nsb_stimulus_drive(const void* tokens, int32_t token_bytes, const nsb_matrix* table, float scale,
+                       const nsb_matrix* out, void* stream) {
+  nsb::Dense t, o;
+  if (!check_matrix(table, &t, "the stimulus table must be a [rows, neurons] matrix of float32, float16 or bfloat16", "the stimulus table is required") ||
+      !check_matrix(out, &o, "the drive must be a [tokens, neurons] matrix of float32, float16 or bfloat16", "the drive output is required"))
+    return NSB_ERR_ARGUMENT;
+  if (o.cols != t.cols) return nsb::set_error(NSB_ERR_ARGUMENT, "drive and table must have the same number of neurons");
+  if (o.type != t.type && o.type != NSB_VALUE_F32) return nsb::set_error(NSB_ERR_ARGUMENT, "the drive has the table's type or float32");
+  if (!check_tokens(tokens, token_bytes, o.rows)) return NSB_ERR_ARGUMENT;
+  nsb::set_error(NSB_OK, "");
+  if (o.rows == 0) return NSB_OK;
+  return done(nsb::launch_stimulus_drive(tokens, token_bytes, o.rows, t, scale, o, static_cast<cudaStream_t>(stream)),
+              "nsb_stimulus_drive launch");
+}
+
+size_t nsb_stimulus_gradient_workspace_size(int64_t tokens, int64_t cols) {
+  if (tokens <= 0 || cols < 1 || tokens >= kMost || cols >= kMost) return 0;
+  return nsb::stimulus_gradient_workspace_bytes(tokens, cols);
+}
+
+int nsb_stimulus_gradient(const void* tokens, int32_t token_bytes, const nsb_matrix* grad, float scale,
+                          const nsb_matrix* out, void* workspace, size_t workspace_bytes, void* stream) {
+  nsb::Dense g, o;
+  if (!check_matrix(grad, &g, "the drive's gradient must be a [tokens, neurons] matrix of float32, float16 or bfloat16", "the drive's gradient is required") ||
+      !check_matrix(out, &o, "the table's gradient must be a [rows, neurons] matrix of float32, float16 or bfloat16", "the table's gradient is required"))
+    return NSB_ERR_ARGUMENT;
+  if (o.cols != g.cols) return nsb::set_error(NSB_ERR_ARGUMENT, "the gradients must have the same number of neurons");
+  if (o.type != g.type && o.type != NSB_VALUE_F32 && g.type != NSB_VALUE_F32)
+    return nsb::set_error(NSB_ERR_ARGUMENT, "one of the gradients must be float32 where their types differ");
+  if (!check_tokens(tokens, token_bytes, g.rows)) return NSB_ERR_ARGUMENT;
+  if (!check_workspace(workspace, workspace_bytes, nsb_stimulus_gradient_workspace_size(g.rows, g.cols), 16)) return NSB_ERR_WORKSPACE;
+  nsb::set_error(NSB_OK, "");
+  if (o.rows == 0) return NSB_OK;
+  return done(nsb::launch_stimulus_gradient(tokens, token_bytes, g, scale, o, workspace, static_cast<cudaStream_t>(stream)),
+              "nsb_stimulus_gradient launch");
+}
+
+size_t nsb_nvfp4_quantize_workspace_size(int64_t rows, int64_t cols, int32_t transpose, int64_t scale_count) {
+  if (rows < 1 || cols < 1 || rows >= kMost || cols >= kMost) return 0;
+  const nsb::Nvfp4 out{transpose ? cols : rows, transpose ? rows : cols, nullptr, 0, nullptr, nullptr, scale_count != 1};
+  return nsb::nvfp4_quantize_workspace_bytes(out, transpose != 0);
+}
+
+int nsb_nvfp4_quantize(const nsb_matrix* value, int32_t transpose, const nsb_nvfp4* out, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+  nsb::Dense v;
+  nsb::Nvfp4 o;
+  if (!check_matrix(value, &v, "the value must be a matrix of float32, float16 or bfloat16", "the value is required") ||
+      !check_nvfp4(out, &o))
+    return NSB_ERR_ARGUMENT;
+  if (o.rows != (transpose ? v.cols : v.rows) || o.cols != (transpose ? v.rows : v.cols))
+    return nsb::set_error(NSB_ERR_ARGUMENT, "the NVFP4 matrix must have the value's shape, or the transposed one");
+  const size_t need = nsb_nvfp4_quantize_workspace_size(v.rows, v.cols, transpose, out->scale_count);
+  if (!check_workspace(workspace, workspace_bytes, need, 4)) return NSB_ERR_WORKSPACE;
+  nsb::set_error(NSB_OK, "");
+  if (v.rows == 0) return NSB_OK;
+  return done(nsb::launch_nvfp4_quantize(v, transpose != 0, o, workspace, static_cast<cudaStream_t>(stream)),
+              "nsb_nvfp4_quantize launch");
+}
+
+int nsb_nvfp4_dequantize(const nsb_nvfp4* value, const nsb_matrix* out, void* stream) {
+  nsb::Nvfp4 v;
+  nsb::Dense o;
+  if (!check_nvfp4(value, &v) ||
+      !check_matrix(out, &o, "the output must be a matrix of float32, float16 or bfloat16", "the output is required"))
+    return NSB_ERR_ARGUMENT;
+  if (o.rows != v.rows || o.cols != v.cols) return nsb::set_error(NSB_ERR_ARGUMENT, "the output must have the NVFP4 matrix's shape");
+  nsb::set_error(NSB_OK, "");
+  if (v.rows == 0) return NSB_OK;
+  return done(nsb::launch_nvfp4_dequantize(v, o, static_cast<cudaStream_t>(stream)), "nsb_nvfp4_dequantize launch");
+}
+
+int nsb_nvfp4_product(const nsb_nvfp4* a, const nsb_nvfp4* b, const float* bias, const nsb_matrix* out,
+                      int* status, void* stream) {
+  nsb::Nvfp4 x, y;
+  nsb::Dense o;
+  if (!check_nvfp4(a, &x) || !check_nvfp4(b, &y) ||
+      !check_matrix(out, &o, "the product must be a matrix of float32, float16 or bfloat16", "the product is required"))
+    return NSB_ERR_ARGUMENT;
+  if (x.cols != y.cols) return nsb::set_error(NSB_ERR_ARGUMENT, "the operands must have the same number of columns");
+  if (y.rows < 1 || o.rows != x.rows || o.cols != y.rows)
+    return nsb::set_error(NSB_ERR_ARGUMENT, "the product must be [a.rows, b.rows], b.rows >= 1");
+  if (reinterpret_cast<uintptr_t>(bias) % 4 != 0) return nsb::set_error(NSB_ERR_ARGUMENT, "the bias must be 4-byte aligned");
+  nsb::set_error(NSB_OK, "");
+  if (x.rows == 0) return NSB_OK;
+  return done(nsb::launch_nvfp4_product(x, y, bias, o, status, static_cast<cudaStream_t>(stream)),
+              "nsb_nvfp4_product launch");
+}
+
+size_t nsb_column_sums_workspace_size(int64_t rows, int64_t cols) {
+  if (rows < 1 || cols < 1 || rows >= kMost || cols >= kMost) return 0;
+  return nsb::column_sums_workspace_bytes(rows, cols);
+}
+
+int nsb_column_sums(const nsb_matrix* value, float* out, void* workspace, size_t workspace_bytes,
+                    void* stream) {
+  nsb::Dense v;
+  if (!check_matrix(value, &v, "the value must be a matrix of float32, float16 or bfloat16", "the value is required"))
+    return NSB_ERR_ARGUMENT;
+  if (!out || reinterpret_cast<uintptr_t>(out) % 4 != 0) return nsb::set_error(NSB_ERR_ARGUMENT, "the sums are required, 4-byte aligned");
+  if (!check_workspace(workspace, workspace_bytes, nsb_column_sums_workspace_size(v.rows, v.cols), 4)) return NSB_ERR_WORKSPACE;
+  nsb::set_error(NSB_OK, "");
+  return done(nsb::launch_column_sums(v, out, workspace, static_cast<cudaStream_t>(stream)), "nsb_column_sums launch");
+}
+
+int nsb_adjust_logits(const nsb_logits* args, void* stream) {
+  if (!args) return nsb::set_error(NSB_ERR_ARGUMENT, "logit arguments are required");
+  nsb::LogitsArgs a{};
+  if (!check_matrix(&args->logits, &a.logits, "logits must be a [rows, vocabulary] matrix of float32, float16 or bfloat16", "logits are required") ||
+      !check_matrix(&args->out, &a.out, "the output must be a [rows, vocabulary] matrix of the logits' type", "the output is required"))
+    return NSB_ERR_ARGUMENT;
+  if (a.out.rows != a.logits.rows || a.out.cols != a.logits.cols || a.out.type != a.logits.type)
+    return nsb::set_error(NSB_ERR_ARGUMENT, "the output must have the logits' shape and type");
+  if (args->history_length < 0 || args->history_length >= kMost || (args->history_length > 0 && a.logits.rows > 0 && (!args->history || args->history_stride < 0)))
+    return nsb::set_error(NSB_ERR_ARGUMENT, "the history must be [rows, length] int32");
+  if ((args->bias && args->bias_stride < 0) || (args->mask && args->mask_stride < 0) ||
+      args->repetition.stride < 0 || args->presence.stride < 0 || args->frequency.stride < 0)
+    return nsb::set_error(NSB_ERR_ARGUMENT, "strides must not be negative");
+  if (!args->repetition.data && !(args->repetition.scalar > 0.0f))
+    return nsb::set_error(NSB_ERR_ARGUMENT, "the repetition penalty must be above 0");
+  a.history = args->history;
+  a.history_length = args->history_length;
+  a.history_stride = args->history_stride;
+  a.lengths = args->lengths;
+  a.prompt_lengths = args->prompt_lengths;
+  a.repetition = args->repetition;
+  a.presence = args->presence;
+  a.frequency = args->frequency;
+  a.bias = args->bias;
+  a.bias_stride = args->bias_stride;
+  a.mask = args->mask;
+  a.mask_stride = args->mask_stride;
+  a.choice = args->choice;
+  nsb::set_error(NSB_OK, "");
+  if (a.logits.rows == 0) return NSB_OK;
+  return done(nsb::launch_adjust_logits(a, static_cast<cudaStream_t>(stream)), "nsb_adjust_logits launch");
+}
+
+}  // extern "C"

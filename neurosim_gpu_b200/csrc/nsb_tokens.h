@@ -1,0 +1,57 @@
+// nsb_tokens.h -- host-side launchers of the token operators, shared with their C ABI (capi_tokens.cu).
+#pragma once
+
+#include "nsb_launch.h"
+#include "nsb_values.cuh"
+
+namespace nsb {
+
+// Records `message` for nsb_last_error() (capi.cu) and returns `code`; never throws.
+int set_error(int code, const char* message) noexcept;
+int set_cuda_error(cudaError_t err, const char* where) noexcept;
+
+// stimulus.cu
+cudaError_t launch_stimulus_drive(const void* tokens, int token_bytes, int64_t n, const Dense& table,
+                                  float scale, const Dense& out, cudaStream_t stream);
+size_t stimulus_gradient_workspace_bytes(int64_t n, int64_t cols);
+cudaError_t launch_stimulus_gradient(const void* tokens, int token_bytes, const Dense& grad,
+                                     float scale, const Dense& out, void* workspace,
+                                     cudaStream_t stream);
+
+// microscale.cu
+struct Nvfp4 {
+  int64_t rows, cols;
+  uint8_t* codes;         // [rows, pitch]
+  int64_t pitch;          // bytes: 16 * ceil(cols / 32)
+  uint8_t* block_scales;  // [ceil(rows / 128), 4 * ceil(cols / 256), 512]
+  float* scale;           // [rows] or [1]
+  bool per_row;
+};
+size_t nvfp4_quantize_workspace_bytes(const Nvfp4& out, bool transpose);
+cudaError_t launch_nvfp4_quantize(const Dense& value, bool transpose, const Nvfp4& out,
+                                  void* workspace, cudaStream_t stream);
+cudaError_t launch_nvfp4_dequantize(const Nvfp4& in, const Dense& out, cudaStream_t stream);
+size_t column_sums_workspace_bytes(int64_t rows, int64_t cols);
+cudaError_t launch_column_sums(const Dense& value, float* out, void* workspace, cudaStream_t stream);
+
+// microscale_product.cu
+cudaError_t launch_nvfp4_product(const Nvfp4& a, const Nvfp4& b, const float* bias, const Dense& out,
+                                 int* status, cudaStream_t stream);
+
+// logits.cu
+struct LogitsArgs {
+  Dense logits, out;
+  const int32_t* history;  // [rows, history_length], stride history_stride
+  int64_t history_length, history_stride;
+  const int32_t* lengths;         // [rows] or null: all history_length
+  const int32_t* prompt_lengths;  // [rows] or null: none
+  nsb_row_values repetition, presence, frequency;
+  const float* bias;              // [rows or 1, vocabulary]
+  int64_t bias_stride;            // 0: the same for all rows
+  const int32_t* mask;            // [rows or 1, ceil(vocabulary / 32)]
+  int64_t mask_stride;
+  int64_t* choice;                // [rows] or null
+};
+cudaError_t launch_adjust_logits(const LogitsArgs& args, cudaStream_t stream);
+
+}  // namespace nsb

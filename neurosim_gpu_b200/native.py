@@ -116,6 +116,34 @@ class _ScatterRows(ctypes.Structure):
                 ("dst", ctypes.c_void_p), ("weight", ctypes.c_void_p)]
 
 
+class _Matrix(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("rows", ctypes.c_int64), ("cols", ctypes.c_int64),
+                ("row_stride", ctypes.c_int64), ("type", ctypes.c_int32)]
+
+
+class _Nvfp4(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("cols", ctypes.c_int64), ("codes", ctypes.c_void_p),
+                ("code_stride", ctypes.c_int64), ("block_scales", ctypes.c_void_p),
+                ("scale", ctypes.c_void_p), ("scale_count", ctypes.c_int64)]
+
+
+class _RowValues(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("stride", ctypes.c_int64), ("scalar", ctypes.c_float)]
+
+
+class _Logits(ctypes.Structure):
+    _fields_ = [("logits", _Matrix), ("out", _Matrix), ("history", ctypes.c_void_p),
+                ("history_length", ctypes.c_int64), ("history_stride", ctypes.c_int64),
+                ("lengths", ctypes.c_void_p), ("prompt_lengths", ctypes.c_void_p),
+                ("repetition", _RowValues), ("presence", _RowValues), ("frequency", _RowValues),
+                ("bias", ctypes.c_void_p), ("bias_stride", ctypes.c_int64),
+                ("mask", ctypes.c_void_p), ("mask_stride", ctypes.c_int64),
+                ("choice", ctypes.c_void_p)]
+
+
+# Values of the token operators (nsb_value_type).
+VALUE_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
 EVENT_ROWS_WORKSPACE = 256
 
 
@@ -138,7 +166,11 @@ EXPORTED_SYMBOLS = ("nsb_dendritic_step", "nsb_csr_propagate",
                     "nsb_dendritic_event_hybrid", "nsb_dendritic_rollout_tiled",
                     "nsb_dendritic_rollout_tiled_peers", "nsb_dendritic_rollout_cluster",
                     "nsb_dendritic_event_rows_gated", "nsb_event_scatter_rows_gated",
-                    "nsb_tiled_propagate_rows_gated", "nsb_last_error", "nsb_abi_version")
+                    "nsb_tiled_propagate_rows_gated", "nsb_stimulus_drive",
+                    "nsb_stimulus_gradient_workspace_size", "nsb_stimulus_gradient",
+                    "nsb_nvfp4_quantize_workspace_size", "nsb_nvfp4_quantize",
+                    "nsb_nvfp4_dequantize", "nsb_nvfp4_product", "nsb_column_sums_workspace_size",
+                    "nsb_column_sums", "nsb_adjust_logits", "nsb_last_error", "nsb_abi_version")
 
 
 @functools.lru_cache(maxsize=1)
@@ -225,11 +257,26 @@ def load_library() -> ctypes.CDLL:
         p(_Tick), ctypes.c_void_p, p(_View), ctypes.c_void_p, ctypes.c_int64, p(_OutCsr),
         p(_TiledLayout), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_uint64,
         p(_TickOut), p(_Out), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_void_p]
+    i32, i64, size, ptr = ctypes.c_int32, ctypes.c_int64, ctypes.c_size_t, ctypes.c_void_p
+    lib.nsb_stimulus_drive.argtypes = [ptr, i32, p(_Matrix), ctypes.c_float, p(_Matrix), ptr]
+    lib.nsb_stimulus_gradient_workspace_size.argtypes = [i64, i64]
+    lib.nsb_stimulus_gradient_workspace_size.restype = size
+    lib.nsb_stimulus_gradient.argtypes = [ptr, i32, p(_Matrix), ctypes.c_float, p(_Matrix), ptr,
+                                          size, ptr]
+    lib.nsb_nvfp4_quantize_workspace_size.argtypes = [i64, i64, i32, i64]
+    lib.nsb_nvfp4_quantize_workspace_size.restype = size
+    lib.nsb_nvfp4_quantize.argtypes = [p(_Matrix), i32, p(_Nvfp4), ptr, size, ptr]
+    lib.nsb_nvfp4_dequantize.argtypes = [p(_Nvfp4), p(_Matrix), ptr]
+    lib.nsb_nvfp4_product.argtypes = [p(_Nvfp4), p(_Nvfp4), ptr, p(_Matrix), ptr, ptr]
+    lib.nsb_column_sums_workspace_size.argtypes = [i64, i64]
+    lib.nsb_column_sums_workspace_size.restype = size
+    lib.nsb_column_sums.argtypes = [p(_Matrix), ptr, ptr, size, ptr]
+    lib.nsb_adjust_logits.argtypes = [p(_Logits), ptr]
     lib.nsb_last_error.restype = ctypes.c_char_p
     lib.nsb_abi_version.restype = ctypes.c_int
     for name in EXPORTED_SYMBOLS:
         getattr(lib, name).restype = getattr(lib, name).restype or ctypes.c_int
-    if lib.nsb_abi_version() != 14:
+    if lib.nsb_abi_version() != 15:
         raise RuntimeError("libneurosim_b200.so ABI version mismatch")
     return lib
 
@@ -268,6 +315,31 @@ def _check(ok: bool, message: str) -> None:
 def _raise_on_status(lib: ctypes.CDLL, status: int) -> None:
     if status != 0:
         raise RuntimeError(lib.nsb_last_error().decode() or f"libneurosim_b200 status {status}")
+
+
+def dense_matrix(value: torch.Tensor, name: str) -> _Matrix:
+    """The C view of a [rows, columns] CUDA tensor with contiguous rows (token operators)."""
+    kind = VALUE_TYPES.get(value.dtype)
+    if kind is None or not value.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor of float32, float16 or bfloat16")
+    if value.dim() != 2:
+        raise ValueError(f"{name} must have two dimensions")
+    rows, cols = value.shape
+    row_stride, stride = value.stride()
+    if rows > 0 and ((cols > 1 and stride != 1) or (rows > 1 and row_stride < cols)):
+        raise ValueError(f"{name} must have contiguous rows that do not overlap")
+    return _Matrix(value.data_ptr(), rows, cols, max(row_stride, cols), kind)
+
+
+def token_call(device: torch.device, function, *arguments) -> None:
+    """Call a token operator of the library on the current stream of ``device``."""
+    if device.index == torch.cuda.current_device():
+        status = function(*arguments, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            status = function(*arguments, torch.cuda.current_stream(device).cuda_stream)
+    if status != 0:
+        _raise_on_status(load_library(), status)
 
 
 def _float_on(value: torch.Tensor, state: torch.Tensor) -> None:

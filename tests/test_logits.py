@@ -1,0 +1,213 @@
+"""Logit penalties, biases, masks and the greedy choice against a plain implementation."""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from neurosim_gpu_b200 import adjust_logits, native
+
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def generator(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def plain(logits, history=None, lengths=None, prompts=None, repetition=1.0, presence=0.0, frequency=0.0,
+          bias=None, mask=None, kind=np.float64):
+    """The formula on the CPU, each step in `kind`; -> (adjusted [B, V] before the last rounding, counts)."""
+    x = logits.float().numpy().astype(kind)
+    rows, vocabulary = x.shape
+    count = np.zeros((rows, vocabulary), np.int64)
+    seen = np.zeros((rows, vocabulary), bool)
+    if history is not None:
+        h = history.numpy()
+        for b in range(rows):
+            end = h.shape[1] if lengths is None else min(max(int(lengths[b]), 0), h.shape[1])
+            start = 0 if prompts is None else int(prompts[b])
+            for i, v in enumerate(h[b, :end]):
+                if 0 <= v < vocabulary:
+                    seen[b, v] = True
+                    count[b, v] += i >= start
+
+    def column(value):
+        value = value.numpy() if isinstance(value, torch.Tensor) else np.float32(value)
+        return np.broadcast_to(np.asarray(value, np.float32).astype(kind).reshape(-1, 1), (rows, 1))
+
+    r, p, f = column(repetition), column(presence), column(frequency)
+    with np.errstate(invalid="ignore"):
+        x = np.where(seen, np.where(x > 0, x / r, x * r), x)
+        x = np.where(count > 0, x - f * count.astype(kind) - p, x)
+        if bias is not None:
+            x = x + bias.numpy().astype(kind)
+    if mask is not None:
+        bits = (mask.numpy().astype(np.uint32)[..., None] >> np.arange(32, dtype=np.uint32)) & 1
+        bits = bits.reshape(*mask.shape[:-1], 32 * mask.shape[-1])[..., :vocabulary]
+        x = np.where(bits == 0, -math.inf, x)
+    return x, count
+
+
+def choice_of(adjusted):
+    x = np.where(np.isnan(adjusted), -math.inf, adjusted)
+    best = x.argmax(1)  # the lowest index of equal ones
+    return np.where(x.max(1) > -math.inf, best, -1)
+
+
+def check(logits, dtype, **kw):
+    names = {"prompts": "prompt_lengths"}
+    device = {names.get(k, k): v.cuda() if isinstance(v, torch.Tensor) else v for k, v in kw.items()}
+    got, choice = adjust_logits(logits.cuda(), choose=True, **device)
+    steps, _ = plain(logits, kind=np.float32, **kw)
+    want = torch.from_numpy(steps).to(dtype)
+    assert got.dtype == dtype
+    torch.testing.assert_close(got.cpu(), want, rtol=0, atol=0, equal_nan=True)  # the same float32 steps
+    assert choice.cpu().tolist() == choice_of(want.float().numpy()).tolist()
+    # ... and near the formula in float64: five float32 roundings of numbers no larger than the
+    # parts' sizes, and the rounding to dtype.
+    exact, count = plain(logits, **kw)
+    size = np.abs(np.nan_to_num(logits.double().numpy())) * 2 + 2 + 2 * count
+    if kw.get("bias") is not None:
+        size = size + np.abs(np.nan_to_num(kw["bias"].numpy(), neginf=0.0))
+    unit = {torch.float32: 0.0, torch.float16: 2.0**-11, torch.bfloat16: 2.0**-8}[dtype]
+    finite = np.isfinite(exact) & np.isfinite(got.float().cpu().numpy())
+    with np.errstate(invalid="ignore"):
+        error = np.abs(got.float().cpu().numpy().astype(np.float64) - exact)
+    bound = 5 * 2.0**-24 * size + unit * np.abs(np.where(finite, exact, 0.0)) + 2.0**-24
+    assert bool((error <= bound)[finite].all())
+    assert np.array_equal(finite, np.isfinite(exact))
+    return got, choice
+
+
+def case(rows, vocabulary, length, seed=0):
+    g = generator(seed)
+    history = torch.randint(-2, vocabulary + 2, (rows, length), generator=g, dtype=torch.int32)
+    if length:
+        history[:, ::3] = history[:, ::3] % max(1, vocabulary // 50 + 1)  # some tokens repeat often
+    return {
+        "history": history,
+        "lengths": torch.randint(-1, length + 3, (rows,), generator=g, dtype=torch.int32),
+        "prompts": torch.randint(0, length + 1, (rows,), generator=g, dtype=torch.int32),
+        "repetition": 1 + torch.rand(rows, generator=g), "presence": torch.rand(rows, generator=g),
+        "frequency": torch.rand(rows, generator=g) - 0.3,
+        "bias": torch.randn(vocabulary, generator=g),
+        "mask": torch.randint(-(2**31), 2**31, (rows, (vocabulary + 31) // 32), generator=g).int(),
+    }
+
+
+def test_entry_point_refuses_bad_arguments():
+    lib = native.load_library()
+    p = 0x1000  # never read: the checks fail first
+
+    def call(**kw):
+        args = native._Logits()
+        args.logits = args.out = native._Matrix(p, 2, 100, 100, 0)
+        args.repetition.scalar = 1.0
+        for name, value in kw.items():
+            setattr(args, name, value)
+        return lib.nsb_adjust_logits(ctypes.byref(args), None)
+
+    for bad in ({"out": native._Matrix(p, 2, 99, 100, 0)}, {"out": native._Matrix(p, 2, 100, 100, 1)},
+                {"logits": native._Matrix(None, 2, 100, 100, 0)}, {"history_length": 5}, {"history_length": -1},
+                {"bias": p, "bias_stride": -1}, {"mask": p, "mask_stride": -1},
+                {"repetition": native._RowValues(None, 0, 0.0)}, {"presence": native._RowValues(p, -1, 0.0)}):
+        assert call(**bad) == -1, bad
+        assert lib.nsb_last_error()
+    assert lib.nsb_adjust_logits(None, None) == -1
+    empty = native._Matrix(None, 0, 100, 100, 0)
+    assert call(logits=empty, out=empty) == 0
+
+
+def test_function_refuses_cpu_tensors():
+    with pytest.raises(ValueError, match="CUDA"):
+        adjust_logits(torch.zeros(2, 8))
+
+
+@pytest.mark.gpu
+def test_function_refuses_bad_arguments():
+    x = torch.zeros(2, 40, device="cuda")
+    words = torch.zeros(2, 2, dtype=torch.int32, device="cuda")
+    for bad in ({"history": words.long()}, {"history": words[:1]}, {"lengths": words[:, 0].contiguous()},
+                {"history": words, "lengths": words[0, :1]}, {"bias": x[0, :39]}, {"bias": x[0].half()},
+                {"mask": words[:, :1]}, {"mask": words.float()}, {"repetition": 0.0}, {"presence": x[:, 0].double()},
+                {"frequency": torch.zeros(3, device="cuda")}, {"out": x[:1]}, {"out": x.half()}):
+        with pytest.raises((ValueError, RuntimeError)):
+            adjust_logits(x, **bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocabulary,length", [(0, 5, 3), (1, 1, 0), (1, 1, 4), (2, 31, 1), (1, 33, 17), (3, 1000, 0),
+                                                    (5, 4097, 300), (2, 70_001, 5000), (1, 131_072, 64)])
+def test_adjust(dtype, rows, vocabulary, length):
+    logits = (3 * torch.randn(rows, vocabulary, generator=generator(1))).to(dtype)
+    check(logits, dtype, **case(rows, vocabulary, length))
+
+
+@pytest.mark.gpu
+def test_every_part_alone():
+    rows, vocabulary = 3, 515
+    logits = torch.randn(rows, vocabulary, generator=generator(2))
+    full = case(rows, vocabulary, 200)
+    check(logits, torch.float32)
+    check(logits, torch.float32, bias=full["bias"])
+    check(logits, torch.float32, mask=full["mask"])
+    check(logits, torch.float32, mask=full["mask"][0], bias=torch.randn(rows, vocabulary))
+    check(logits, torch.float32, history=full["history"], repetition=1.3)
+    check(logits, torch.float32, history=full["history"], presence=0.5)
+    check(logits, torch.float32, history=full["history"], lengths=full["lengths"], frequency=0.25, presence=-0.5)
+    check(logits, torch.float32, history=full["history"], prompts=full["prompts"], repetition=0.5, frequency=1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_masked_rows_ties_and_values_that_are_not_finite(dtype):
+    vocabulary = 9001
+    logits = torch.zeros(6, vocabulary, dtype=dtype)
+    mask = torch.full((6, (vocabulary + 31) // 32), -1, dtype=torch.int32)
+    mask[0] = 0                                    # nothing left
+    mask[1] = 0
+    mask[1, 200] = 1 << 5                          # one token left
+    logits[2, [70, 8999, 9000]] = 2.0              # equal largest: the lowest index
+    logits[3] = torch.finfo(dtype).min             # the type's lowest value is still a choice
+    logits[4, 10] = math.nan                       # never chosen
+    logits[4, 20] = math.inf
+    logits[5] = -math.inf
+    for value in (math.nan, math.inf):             # in masked places they vanish
+        logits[1, 7] = value
+        got, choice = check(logits, dtype, mask=mask)
+        assert choice.tolist() == [-1, 200 * 32 + 5, 70, 0, 20, -1]
+        assert bool(torch.isneginf(got[0]).all()) and int(torch.isfinite(got[1]).sum()) == 1
+    bias = torch.zeros(vocabulary)
+    bias[70] = -math.inf                           # a bias can ban a token
+    assert check(logits, dtype, mask=mask, bias=bias)[1].tolist()[2] == 8999
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_strided_rows_in_place_and_graph(dtype):
+    rows, vocabulary = 4, 3001
+    kw = case(rows, vocabulary, 90)
+    base = torch.randn(rows * 3100 + 8, generator=generator(3)).to(dtype)
+    for offset, stride in ((0, 3001), (1, 3008), (3, 3013), (8, 3024)):
+        view = base.as_strided((rows, vocabulary), (stride, 1), offset)
+        got, _ = check(view.clone(), dtype, **kw)
+        device = {("prompt_lengths" if k == "prompts" else k): v.cuda() for k, v in kw.items()}
+        strided = base.cuda().as_strided((rows, vocabulary), (stride, 1), offset)
+        assert torch.equal(adjust_logits(strided, **device), got)
+        out = torch.zeros(rows, 3030, dtype=dtype, device="cuda")[:, 2:3003]  # another place within 16 bytes
+        assert torch.equal(adjust_logits(strided, out=out, **device), got)
+        assert adjust_logits(strided, out=strided, **device) is strided
+        assert torch.equal(strided, got)
+    source = base[: rows * vocabulary].view(rows, vocabulary).cuda()
+    want, choice = adjust_logits(source, choose=True, **device)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a, b = adjust_logits(source, choose=True, **device)
+    a.zero_(), b.zero_()
+    graph.replay()
+    assert torch.equal(a, want) and torch.equal(b, choice)

@@ -1,0 +1,400 @@
+"""NVFP4 matrices, their product and the readout against plain implementations in float64."""
+
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from neurosim_gpu_b200 import (Nvfp4Matrix, check_product_status, native, nvfp4_product, nvfp4_readout,
+                               quantize_dequantize, quantize_nvfp4)
+
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+UNIT = {torch.float32: 2.0**-24, torch.float16: 2.0**-11, torch.bfloat16: 2.0**-8}
+LEVELS = np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6, 0, -0.5, -1, -1.5, -2, -3, -4, -6])
+
+
+def generator(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def blocks_of(x):
+    rows, columns = x.shape
+    out = np.zeros((rows, (columns + 15) // 16 * 16), np.float64)
+    out[:, :columns] = x
+    return out.reshape(rows, -1, 16)
+
+
+def e4m3(x):
+    """The E4M3 number nearest to x >= 0 (ties to even, at most 448), in float64."""
+    x = np.asarray(x, np.float64)
+    exponent = np.maximum(np.floor(np.log2(np.maximum(x, 2.0**-60))), -6)
+    unit = 2.0 ** (exponent - 3)
+    return np.minimum(np.round(x / unit) * unit, 448.0)
+
+
+def quantized(x, per):
+    """(values [R, K], block scales [R, blocks], scale) of the format's definition; the quotients
+    that decide are float32 ones."""
+    b = blocks_of(x.double().numpy())
+    amax = np.abs(b).max((1, 2)) if per == "row" else np.full(len(b), np.abs(b).max())
+    scale = np.maximum((amax.astype(np.float32) / np.float32(2688)), np.float32(2.0**-126))
+    s = scale[:, None].astype(np.float32)
+    block = e4m3(np.minimum(np.abs(b).max(2).astype(np.float32) / (np.float32(6) * s), np.float32(448)))
+    step = s * block.astype(np.float32)
+    ratio = np.abs(b).astype(np.float32) / np.where(step > 0, step, np.float32(1))[..., None]
+    ratio = ratio.astype(np.float64)
+    # Levels are 0.5 apart below 2, 1 apart below 4, then 2 apart: numpy rounds ties to even multiples.
+    level = np.where(ratio < 2, np.round(ratio * 2) / 2, np.where(ratio < 4, np.round(ratio), np.round(ratio / 2) * 2))
+    value = np.copysign(np.minimum(level, 6), b) * (block * s)[..., None].astype(np.float64)
+    return value.reshape(len(b), -1)[:, : x.shape[1]], block, scale
+
+
+def untiled(packed):
+    tiles = packed.block_scales.cpu()
+    flat = tiles.view(*tiles.shape[:2], 32, 4, 4).permute(0, 3, 2, 1, 4).reshape(tiles.shape[0] * 128, -1)
+    return flat.contiguous()
+
+
+def check_packed(packed, x, per):
+    """Codes, block scales, scale, padding and what is read back."""
+    value, block, scale = quantized(x, per)
+    rows, columns = x.shape
+    assert packed.shape == (rows, columns)
+    assert np.array_equal(packed.scale.cpu().numpy(), scale if per == "row" else scale[:1])
+    got = untiled(packed)
+    want = torch.zeros_like(got)
+    want[:rows, : block.shape[1]] = torch.from_numpy(block).float().to(torch.float8_e4m3fn).view(torch.uint8)
+    assert torch.equal(got, want)  # zeros beyond the matrix, too
+    codes = packed.codes.cpu().numpy()
+    codes = np.stack([codes & 15, codes >> 4], -1).reshape(rows, -1)
+    assert not codes[:, columns:].any()
+    step = np.repeat(block * packed.scale.cpu().numpy().astype(np.float32).reshape(-1, 1).astype(np.float64), 16, 1)[:, :columns]
+    decoded = LEVELS[codes[:, :columns]] * step
+    assert np.array_equal(decoded, value)
+    assert np.array_equal(np.signbit(LEVELS[codes[:, :columns]]) | (codes[:, :columns] == 8), np.signbit(x.float().numpy()))
+    # Read back: level * (block scale * scale), both products rounded to float32, then to the type.
+    for dtype in DTYPES:
+        back = packed.dequantize(dtype)
+        want = torch.from_numpy(LEVELS[codes[:, :columns]].astype(np.float32) * step.astype(np.float32)).to(dtype)
+        assert torch.equal(back.cpu(), want)
+
+
+# -- refusals -------------------------------------------------------------------------------------
+
+
+def test_entry_points_refuse_bad_arguments():
+    lib = native.load_library()
+    p = 0x1000  # never read: the checks fail first
+    value = native._Matrix(p, 4, 40, 40, 0)
+
+    def packed(rows=4, cols=40, codes=p, stride=32, scales=p, scale=p, count=1):
+        return native._Nvfp4(rows, cols, codes, stride, scales, scale, count)
+
+    def quantize(value=value, transpose=0, out=None, workspace=p, size=4):
+        return lib.nsb_nvfp4_quantize(ctypes.byref(value), transpose, ctypes.byref(out or packed()), workspace, size, None)
+
+    for bad in (packed(rows=5), packed(cols=41), packed(stride=16), packed(codes=p + 8), packed(scales=None),
+                packed(scale=p + 2), packed(count=3), packed(codes=None), packed(rows=-1), packed(cols=0, stride=0)):
+        assert quantize(out=bad) == -1
+        assert lib.nsb_last_error()
+    assert quantize(transpose=1) == -1 and quantize(value=native._Matrix(p, 4, 40, 40, 7)) == -1
+    assert quantize(workspace=None) == -3 and quantize(size=3) == -3 and quantize(workspace=p + 2) == -3
+    out = native._Matrix(p, 4, 6, 6, 0)
+
+    def product(a=None, b=None, out=out, bias=None):
+        return lib.nsb_nvfp4_product(ctypes.byref(a or packed()), ctypes.byref(b or packed(rows=6)), bias,
+                                     ctypes.byref(out), None, None)
+
+    for bad in ({"b": packed(rows=6, cols=41)}, {"b": packed(rows=7)}, {"a": packed(rows=5)}, {"bias": p + 2},
+                {"out": native._Matrix(p, 4, 6, 5, 0)}, {"out": native._Matrix(p + 2, 4, 6, 6, 0)}):
+        assert product(**bad) == -1, bad
+    assert product(a=packed(rows=0, codes=None, scales=None, scale=None),
+                   out=native._Matrix(None, 0, 6, 6, 0)) == 0
+    assert lib.nsb_nvfp4_dequantize(ctypes.byref(packed()), ctypes.byref(native._Matrix(p, 4, 41, 41, 0)), None) == -1
+    assert lib.nsb_column_sums(ctypes.byref(value), None, p, 10**6, None) == -1
+    assert lib.nsb_column_sums(ctypes.byref(value), p, p, 1, None) == -3
+
+
+def test_functions_refuse_cpu_tensors():
+    with pytest.raises(ValueError, match="CUDA"):
+        quantize_nvfp4(torch.zeros(2, 32))
+
+
+@pytest.mark.gpu
+def test_functions_refuse_bad_arguments():
+    x = torch.zeros(4, 40, device="cuda")
+    q = quantize_nvfp4(x)
+    for call in (lambda: quantize_nvfp4(x, per="block"), lambda: quantize_nvfp4(x.double()), lambda: quantize_nvfp4(x[0]),
+                 lambda: quantize_nvfp4(x.t()), lambda: quantize_nvfp4(x[:, :0]), lambda: q.dequantize(torch.float64),
+                 lambda: quantize_nvfp4(x[:0], transpose=True),
+                 lambda: Nvfp4Matrix(q.codes, q.block_scales, q.scale, 70), lambda: Nvfp4Matrix(q.codes, q.block_scales, q.scale[:2], 40),
+                 lambda: Nvfp4Matrix(q.codes, q.block_scales[:, :2], q.scale, 40), lambda: Nvfp4Matrix(q.codes.cpu(), q.block_scales, q.scale, 40),
+                 lambda: nvfp4_product(q, quantize_nvfp4(x[:, :39])), lambda: nvfp4_product(q, q, bias=x[0, :4].half()),
+                 lambda: nvfp4_product(q, q, bias=x[0, :3]), lambda: nvfp4_product(q, q, dtype=torch.float64),
+                 lambda: nvfp4_product(q, q, out=x), lambda: nvfp4_readout(x[:, :39], q),
+                 lambda: nvfp4_readout(x.clone().requires_grad_(), q), lambda: nvfp4_readout(x, q, dtype=torch.int32)):
+        with pytest.raises(ValueError):
+            call()
+
+
+# -- the format -----------------------------------------------------------------------------------
+
+SHAPES = [(1, 1), (1, 16), (2, 15), (3, 17), (1, 257), (130, 255), (257, 48), (128, 256), (5, 1000), (64, 4104), (33, 9000)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,columns", SHAPES)
+def test_quantize(dtype, rows, columns):
+    x = torch.randn(rows, columns, generator=generator(rows)) * torch.exp(2 * torch.randn(rows, 1, generator=generator(1)))
+    x = x.to(dtype)
+    for per in ("row", "tensor"):
+        check_packed(quantize_nvfp4(x.cuda(), per=per), x, per)
+        check_packed(quantize_nvfp4(x.cuda(), per=per, transpose=True), x.t().contiguous(), per)
+
+
+@pytest.mark.gpu
+def test_quantize_strides_ties_and_small_values():
+    g = generator(3)
+    base = torch.randn(60 * 70, generator=g)
+    for offset, stride in ((0, 64), (1, 64), (0, 65), (4, 60)):
+        x = base.as_strided((50, 50), (stride, 1), offset)
+        cuda = base.cuda().as_strided((50, 50), (stride, 1), offset)
+        check_packed(quantize_nvfp4(cuda), x, "row")
+        check_packed(quantize_nvfp4(cuda, per="tensor", transpose=True), x.t(), "tensor")
+    # Scale 1 and block scale 448 or 1: every midpoint of the levels, and values one float32 beside it.
+    middle = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])
+    line = torch.cat([middle, middle.nextafter(torch.tensor(9.0)), middle.nextafter(torch.tensor(0.0)), torch.tensor([6.0, 0.0, -0.0])])
+    x = torch.zeros(3, 64)
+    x[0, 0] = 2688.0
+    x[0, 16:40], x[0, 40:64] = line, -line
+    x[1] = x[0] * 2.0**-100
+    x[2] = x[0] * 2.0**-140  # float32 subnormals: the scale stops at FLT_MIN
+    check_packed(quantize_nvfp4(x.cuda()), x, "row")
+    zeros = torch.zeros(2, 40)
+    zeros[0, 3] = -0.0
+    check_packed(quantize_nvfp4(zeros.cuda()), zeros, "row")
+
+
+@pytest.mark.gpu
+def test_one_scale_gives_the_sparse_weights_values():
+    x = torch.randn(37, 333, generator=generator(4)).cuda()
+    assert torch.equal(quantize_nvfp4(x, per="tensor").dequantize(), quantize_dequantize(x, "nvfp4"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+def test_values_that_are_not_finite_stay_visible(value):
+    x = torch.randn(40, 300, generator=generator(5)).cuda()
+    want = quantize_nvfp4(x).dequantize()
+    x[7, 299] = value
+    back = quantize_nvfp4(x).dequantize()
+    assert bool(back[7].isnan().all())
+    keep = torch.arange(40, device="cuda") != 7
+    assert torch.equal(back[keep], want[keep])
+    back = quantize_nvfp4(x, transpose=True).dequantize()
+    assert bool(back[299].isnan().all()) and not bool(back[:299].isnan().any())
+    assert bool(quantize_nvfp4(x, per="tensor").dequantize().isnan().all())
+    y = nvfp4_readout(x, quantize_nvfp4(want, per="tensor"))
+    assert bool(y[7].isnan().all()) and not bool(y[keep].isnan().any())
+
+
+# -- the product ----------------------------------------------------------------------------------
+
+PRODUCTS = [(1, 1, 1), (1, 1000, 16), (1, 129, 4096), (2, 8, 17), (3, 257, 1000), (8, 1001, 5000), (16, 128, 64), (17, 300, 255),
+            (33, 100, 256), (64, 131, 257), (127, 129, 512), (128, 128, 768), (129, 257, 63), (130, 2, 320), (255, 640, 1024),
+            (256, 256, 2048), (257, 513, 300), (300, 77, 4104), (520, 1030, 272), (1025, 96, 1600)]
+
+
+def exact_operand(rows, columns, seed):
+    """A packed matrix of small integers at scale 1 (block scales 1 or 2), and its values."""
+    g = generator(seed)
+    codes = torch.tensor([0, 2, 4, 10, 12], dtype=torch.uint8)[torch.randint(0, 5, (rows, columns), generator=g)]  # 0 1 2 -1 -2
+    blocks = (columns + 15) // 16
+    twice = torch.randint(0, 2, (rows, blocks), generator=g)
+    value = torch.from_numpy(LEVELS[codes.numpy()]) * torch.repeat_interleave(1 + twice, 16, 1)[:, :columns]
+    wide = torch.zeros(rows, (columns + 31) // 32 * 32, dtype=torch.uint8)
+    wide[:, :columns] = codes
+    scales = torch.zeros((rows + 127) // 128 * 128, (columns + 255) // 256 * 16, dtype=torch.uint8)
+    scales[:rows, :blocks] = 0x38 + 8 * twice.to(torch.uint8)  # E4M3 1.0 and 2.0
+    tiles = scales.view(-1, 4, 32, scales.shape[1] // 4, 4).permute(0, 3, 2, 1, 4).reshape(scales.shape[0] // 128, -1, 512)
+    packed = Nvfp4Matrix((wide[:, 0::2] | (wide[:, 1::2] << 4)).cuda(), tiles.contiguous().cuda(), torch.ones(1, device="cuda"), columns)
+    return packed, value
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", PRODUCTS)
+def test_product_of_integers_is_exact(m, n, k):
+    a, x = exact_operand(m, k, 1)
+    b, y = exact_operand(n, k, 2)
+    assert torch.equal(a.dequantize().cpu().double(), x)
+    bias = torch.randint(-9, 10, (n,), generator=generator(3)).float()
+    want = x @ y.t()  # sums below 2^24: exact in float32 in any order
+    got = nvfp4_product(a, b)
+    assert torch.equal(got.cpu().double(), want)
+    assert torch.equal(nvfp4_product(a, b, bias=bias.cuda()).cpu().double(), want + bias)
+    wide = torch.full((m, n + 5), 7.0, device="cuda")
+    nvfp4_product(a, b, out=wide[:, 1 : n + 1])
+    assert torch.equal(wide[:, 1 : n + 1], got) and bool((wide[:, n + 1 :] == 7).all()) and bool((wide[:, 0] == 7).all())
+    check_product_status()
+
+
+def product_bound(x, y, dtype):
+    """The float64 product and how far it may be off: blocks of 16 are exact in float32, each of the
+    K / 16 additions, at most, loses 2^-23 of the sum of sizes (truncation), the scales three roundings."""
+    want, size = x @ y.t(), x.abs() @ y.abs().t()
+    return want, ((x.shape[1] + 15) // 16 + 4) * 2.0**-23 * size + 2 * UNIT[dtype] * want.abs() + 2.0**-25 * (dtype == torch.float16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", [p for p in PRODUCTS if p[2] > 200])
+def test_product(dtype, m, n, k):
+    a = quantize_nvfp4(torch.randn(m, k, generator=generator(4)).cuda())
+    b = quantize_nvfp4(torch.randn(n, k, generator=generator(5)).cuda() / k**0.5, per="tensor")
+    bias = torch.randn(n, generator=generator(6))
+    x, y = (torch.from_numpy(decode(p)) for p in (a, b))
+    want, bound = product_bound(x, y, dtype)
+    got = nvfp4_product(a, b, bias=bias.cuda(), dtype=dtype)
+    assert got.dtype == dtype
+    error = (got.cpu().double() - (want + bias.double())).abs()
+    assert bool((error <= bound + (2.0**-23 + 2 * UNIT[dtype]) * bias.abs().unsqueeze(0)).all())
+    assert torch.equal(nvfp4_product(a, b, bias=bias.cuda(), dtype=dtype), got)
+    check_product_status()
+
+
+def decode(packed):
+    """The float64 values of a packed matrix, from its bytes."""
+    codes = packed.codes.cpu().numpy()
+    codes = np.stack([codes & 15, codes >> 4], -1).reshape(packed.rows, -1)[:, : packed.columns]
+    scales = untiled(packed)[: packed.rows].view(torch.float8_e4m3fn).double().numpy()
+    step = np.repeat(scales, 16, 1)[:, : packed.columns] * packed.scale.cpu().double().numpy().reshape(-1, 1)
+    return LEVELS[codes] * step
+
+
+@pytest.mark.gpu
+def test_product_of_extreme_scales():
+    """Scales at both ends of float32 and E4M3: the sum is scaled one operand at a time."""
+    g = generator(7)
+    for big, small in ((1e30, 1e-30), (1e-30, 1e20), (1e-38, 1.0)):
+        x, y = big * torch.randn(5, 320, generator=g), small * torch.randn(9, 320, generator=g)
+        x[:, 64:128] *= 1e-3
+        a, b = quantize_nvfp4(x.cuda()), quantize_nvfp4(y.cuda())
+        want, bound = product_bound(torch.from_numpy(decode(a)), torch.from_numpy(decode(b)), torch.float32)
+        assert bool(((nvfp4_product(a, b).cpu().double() - want).abs() <= bound + 2.0**-149).all())
+
+
+@pytest.mark.gpu
+def test_product_on_a_side_stream_and_in_a_graph():
+    x, w = torch.randn(70, 700, generator=generator(8)).cuda(), torch.randn(200, 700, generator=generator(9)).cuda()
+    packed = quantize_nvfp4(w, per="tensor")
+    want = nvfp4_readout(x, packed)
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(20_000_000)
+        later = torch.zeros_like(x)
+        later.copy_(x)
+        got = nvfp4_readout(later, packed)
+    stream.synchronize()
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = nvfp4_readout(x, packed)
+    y.zero_()
+    graph.replay()
+    assert torch.equal(y, want)
+
+
+# -- the readout and its gradients ----------------------------------------------------------------
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape,n", [((1, 300), 40), ((5, 2, 300), 40), ((300,), 7), ((2, 0, 300), 7), ((140, 1000), 333)])
+def test_readout(dtype, shape, n):
+    state = torch.rand(*shape, generator=generator(10)).to(dtype)
+    weight = torch.randn(n, shape[-1], generator=generator(11))
+    bias = torch.randn(n, generator=generator(12))
+    packed = quantize_nvfp4(weight.cuda(), per="tensor")
+    got = nvfp4_readout(state.cuda(), packed, bias.cuda())
+    assert got.shape == (*shape[:-1], n) and got.dtype == dtype
+    flat = state.reshape(-1, shape[-1])
+    if len(flat):
+        want, bound = product_bound(torch.from_numpy(quantized(flat, "row")[0]), torch.from_numpy(quantized(weight, "tensor")[0]), dtype)
+        error = (got.cpu().double().reshape(-1, n) - (want + bias.double())).abs()
+        assert bool((error <= bound + (2.0**-23 + 2 * UNIT[dtype]) * bias.abs()).all())
+    assert torch.equal(nvfp4_readout(state.cuda(), weight.cuda(), bias.cuda()), got)
+    if len(shape) == 2:  # neuron-major states, as the batch tick leaves them
+        assert torch.equal(nvfp4_readout(state.cuda().t().contiguous().t(), packed, bias.cuda()), got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,k,n", [(1, 64, 1), (40, 130, 70), (129, 257, 300), (300, 1024, 128)])
+def test_gradients_match_the_formula(dtype, m, k, n):
+    g = generator(13)
+    x = torch.rand(m, k, generator=g).to(dtype)
+    w = torch.randn(n, k, generator=g).to(dtype)
+    b = torch.randn(n, generator=g)
+    d = torch.randn(m, n, generator=g).to(dtype)
+    leaves = [t.cuda().requires_grad_() for t in (x, w, b)]
+    y = nvfp4_readout(*leaves)
+    grads = torch.autograd.grad(y, leaves, d.cuda())
+
+    def q(t, per):
+        return torch.from_numpy(quantized(t, per)[0])
+
+    for got, left, right in ((grads[0], q(d, "row"), q(w.t(), "tensor")), (grads[1], q(d.t(), "tensor"), q(x.t(), "tensor"))):
+        want, bound = product_bound(left, right, dtype)
+        assert got.dtype == dtype
+        assert bool(((got.cpu().double() - want).abs() <= bound).all())
+    db = d.double().sum(0)
+    assert bool(((grads[2].cpu().double() - db).abs() <= m * 2.0**-24 * d.double().abs().sum(0)).all())
+    with torch.no_grad():
+        assert torch.equal(y.detach(), nvfp4_readout(*leaves))
+
+
+@pytest.mark.gpu
+def test_gradients_match_differences():
+    """On values that NVFP4 holds exactly the readout is the linear map itself, and so are its differences."""
+    g = generator(14)
+    x, w, d = (torch.randint(-1, 2, s, generator=g).double() for s in ((6, 48), (9, 48), (6, 9)))
+    for t in (x, w, d):
+        t[:, ::8] = 6.0  # every block holds its largest level, in both directions of the quantiser
+        t[::6] = 6.0
+        t *= 448.0  # ... so that every scale is 1 and every block scale 448: nothing is rounded anywhere
+    leaves = [t.float().cuda().requires_grad_() for t in (x, w)]
+    bias = torch.zeros(9, device="cuda", requires_grad=True)
+
+    def loss(x, w, b):
+        return (nvfp4_readout(x, w, b) * d.float().cuda()).sum(dtype=torch.float64)
+
+    dx, dw, db = torch.autograd.grad(nvfp4_readout(*leaves, bias), (*leaves, bias), d.float().cuda())
+    with torch.no_grad():
+        for grad, i in ((dx, 0), (dw, 1)):
+            for r, c in ((1, 1), (2, 13), (5, 47)):
+                moved = [leaves[0].clone(), leaves[1].clone()]
+                moved[i][r, c] = 448.0
+                up = loss(*moved, bias)
+                moved[i][r, c] = -448.0
+                assert float(up - loss(*moved, bias)) / 896 == pytest.approx(float(grad[r, c]), rel=1e-6)
+        step = torch.zeros_like(bias)
+        step[4] = 448.0
+        difference = float(loss(*leaves, bias + step) - loss(*leaves, bias)) / 448
+        assert difference == pytest.approx(float(db[4]), rel=1e-6)
+
+
+@pytest.mark.gpu
+def test_gradients_of_some_and_of_empty_batches():
+    x, w = torch.rand(5, 40, device="cuda"), torch.randn(6, 40, device="cuda", requires_grad=True)
+    (dw,) = torch.autograd.grad(nvfp4_readout(x, w).sum(), w)  # an expanded gradient, no bias
+    assert dw.shape == w.shape and bool(dw.any())
+    (dw,) = torch.autograd.grad(nvfp4_readout(x[:0], w).sum(), w)
+    assert not bool(dw.any())
+    b = torch.zeros(6, device="cuda", requires_grad=True)
+    (db,) = torch.autograd.grad(nvfp4_readout(x[:0], w.detach(), b).sum(), b)
+    assert not bool(db.any())
