@@ -1,0 +1,146 @@
+// nsb_tcgen05.cuh -- mbarriers, TMA loads and the fifth-generation tensor core (tcgen05) as inline
+// PTX, for the NVFP4 product.  Every wait is bounded.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace nsb {
+
+__device__ __forceinline__ uint32_t shared_addr(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+
+// ---------------------------------------------------------------------------
+// mbarriers
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void barrier_init(uint64_t* bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(shared_addr(bar)), "r"(count) : "memory");
+}
+
+__device__ __forceinline__ void barrier_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(shared_addr(bar)) : "memory");
+}
+
+__device__ __forceinline__ void barrier_arrive_expect(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(shared_addr(bar)), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ bool barrier_try(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(shared_addr(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+
+// Polls before a wait gives up (tens of milliseconds at the least).
+constexpr int kBarrierPolls = 1 << 22;
+
+// Bounded wait for the phase `parity` of `bar`; gives up at once when another role of the CTA has (`*aborted`).
+__device__ __forceinline__ bool barrier_wait(uint64_t* bar, uint32_t parity, volatile int* aborted) {
+  for (int i = 0; i < kBarrierPolls; ++i) {
+    if (barrier_try(bar, parity)) return true;
+    if ((i & 255) == 255 && *aborted) return false;
+  }
+  return false;
+}
+
+// ---------------------------------------------------------------------------
+// Copies into shared memory (completion counted in bytes on an mbarrier)
+// ---------------------------------------------------------------------------
+// A box of a two-dimensional byte tensor; x (bytes) is a multiple of 16.
+__device__ __forceinline__ void load_box(void* to, const void* map, int x, int y, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+          shared_addr(to)),
+      "l"(map), "r"(x), "r"(y), "r"(shared_addr(bar))
+      : "memory");
+}
+
+// `bytes` consecutive bytes; both addresses and the size are multiples of 16.
+__device__ __forceinline__ void load_bytes(void* to, const void* from, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   shared_addr(to)),
+               "l"(from), "r"(bytes), "r"(shared_addr(bar))
+               : "memory");
+}
+
+// ---------------------------------------------------------------------------
+// Tensor memory: 128 lanes x 512 columns of 32 bits; an address is lane << 16 | column.
+// ---------------------------------------------------------------------------
+// By one whole warp, which also frees it.  The address lands in *slot (shared memory).
+__device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t columns) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_addr(slot)), "r"(columns) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+
+__device__ __forceinline__ void tmem_free(uint32_t address, uint32_t columns) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(address), "r"(columns));
+}
+
+__device__ __forceinline__ void tcgen05_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tcgen05_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// 16 columns of the warp's 32 lanes, one lane per thread; tmem_wait() of them before they are used.
+__device__ __forceinline__ void tmem_load16(uint32_t address, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(address));
+}
+// Waits for the warp's loads.  The values pass through it, so that no use moves ahead of the wait.
+__device__ __forceinline__ void tmem_wait(uint32_t (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]),
+                 "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+               :
+               : "memory");
+}
+
+// ---------------------------------------------------------------------------
+// Shared-memory descriptors: address and strides in units of 16 bytes, bit 46 the descriptor's version.
+// ---------------------------------------------------------------------------
+// Rows of 128 bytes in the 128-byte swizzle (as load_box leaves them), groups of 8 rows 1,024 bytes apart.
+__device__ __forceinline__ uint64_t swizzled_descriptor(uint32_t address) {
+  return static_cast<uint64_t>((address >> 4) & 0x3fff) | (uint64_t{1} << 16) | (uint64_t{64} << 32) | (uint64_t{1} << 46) |
+         (uint64_t{2} << 61);
+}
+// Rows of 16 bytes without a swizzle, groups of 8 rows 128 bytes apart.
+__device__ __forceinline__ uint64_t plain_descriptor(uint32_t address) {
+  return static_cast<uint64_t>((address >> 4) & 0x3fff) | (uint64_t{1} << 16) | (uint64_t{8} << 32) | (uint64_t{1} << 46);
+}
+
+// ---------------------------------------------------------------------------
+// Block-scaled products of E2M1 operands with a UE4M3 scale per 16 elements
+// ---------------------------------------------------------------------------
+// 512 bytes of scales (32 rows of 16 bytes) to 4 columns, in each of the four 32-lane quarters.
+// Ordered before the products that the same thread issues after it.
+__device__ __forceinline__ void copy_scales(uint32_t tmem, uint64_t descriptor) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(descriptor) : "memory");
+}
+
+// The instruction descriptor: E2M1 x E2M1, UE4M3 scales, M = 128 lanes, N columns, both operands K-major.
+__device__ __forceinline__ uint32_t nvfp4_instruction(int n) {
+  return (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+// One thread: D[128, n] (+)= A[128, 64] B[n, 64]^T with the scales at scale_a / scale_b in tensor memory.
+__device__ __forceinline__ void nvfp4_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t instruction, uint32_t scale_a,
+                                          uint32_t scale_b, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(instruction), "r"(scale_a), "r"(scale_b), "r"(accumulate ? 1u : 0u)
+      : "memory");
+}
+
+// Arrives on `bar` once all tcgen05 work that this thread has issued is complete.
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(shared_addr(bar)) : "memory");
+}
+
+}  // namespace nsb
