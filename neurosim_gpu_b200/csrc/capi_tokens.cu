@@ -39,7 +39,7 @@ bool check_nvfp4(const nsb_nvfp4* m, nsb::Nvfp4* d) {
   if (reinterpret_cast<uintptr_t>(m->codes) % 16 != 0 || reinterpret_cast<uintptr_t>(m->block_scales) % 16 != 0 ||
       reinterpret_cast<uintptr_t>(m->scale) % 4 != 0)
     return fail("NVFP4 codes and block scales must be 16-byte aligned, the scale 4-byte aligned");
-  *d = {m->rows, m->cols, m->codes, m->code_stride, m->block_scales, m->scale, m->scale_count != 1};
+  *d = {m->rows, m->cols, m->codes, m->code_stride, m->block_scales, m->scale, m->scale_count == m->rows};
   return true;
 }
 
@@ -97,7 +97,7 @@ int nsb_stimulus_gradient(const void* tokens, int32_t token_bytes, const nsb_mat
 
 size_t nsb_nvfp4_quantize_workspace_size(int64_t rows, int64_t cols, int32_t transpose, int64_t scale_count) {
   if (rows < 1 || cols < 1 || rows >= kMost || cols >= kMost) return 0;
-  const nsb::Nvfp4 out{transpose ? cols : rows, transpose ? rows : cols, nullptr, 0, nullptr, nullptr, scale_count != 1};
+  const nsb::Nvfp4 out{transpose ? cols : rows, transpose ? rows : cols, nullptr, 0, nullptr, nullptr, scale_count == (transpose ? cols : rows)};
   return nsb::nvfp4_quantize_workspace_bytes(out, transpose != 0);
 }
 

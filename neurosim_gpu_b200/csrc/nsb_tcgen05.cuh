@@ -11,6 +11,13 @@ __device__ __forceinline__ uint32_t shared_addr(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
 
+// One thread of a converged warp, the same one each time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t elected;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected));
+  return elected != 0;
+}
+
 // ---------------------------------------------------------------------------
 // mbarriers
 // ---------------------------------------------------------------------------
@@ -84,7 +91,7 @@ __device__ __forceinline__ void tmem_free(uint32_t address, uint32_t columns) {
 __device__ __forceinline__ void tcgen05_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tcgen05_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// 16 columns of the warp's 32 lanes, one lane per thread; tmem_wait() of them before they are used.
+// 16 columns of the warp's 32 lanes, one lane per thread; tmem_wait() before they are used.
 __device__ __forceinline__ void tmem_load16(uint32_t address, uint32_t (&v)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
@@ -92,13 +99,12 @@ __device__ __forceinline__ void tmem_load16(uint32_t address, uint32_t (&v)[16])
         "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
       : "r"(address));
 }
-// Waits for the warp's loads.  The values pass through it, so that no use moves ahead of the wait.
-__device__ __forceinline__ void tmem_wait(uint32_t (&v)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
+// Waits for the warp's loads; then tmem_loaded() of each set, so that no use of its values moves ahead of the wait.
+__device__ __forceinline__ void tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_loaded(uint32_t (&v)[16]) {
+  asm volatile(""
                : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]),
-                 "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
-               :
-               : "memory");
+                 "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]));
 }
 
 // ---------------------------------------------------------------------------
