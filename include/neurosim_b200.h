@@ -595,11 +595,15 @@ typedef struct nsb_nvfp4 {
 } nsb_nvfp4;
 
 /* `out` = the NVFP4 form of `value` (transpose = 0: out->rows = value->rows) or of its transpose.
+ * `amax` (device, may be NULL): the largest |value| of the matrix, as an earlier call on the same
+ * values left it (amax_given != 0; saves the pass that one scale for all rows needs), or to be
+ * written (amax_given = 0; not written for a transpose with a scale per row).
  * Workspace: 4-byte aligned, contents need not be initialised (may be NULL where the size is 0). */
 NSB_API size_t nsb_nvfp4_quantize_workspace_size(int64_t rows, int64_t cols, int32_t transpose,
                                                  int64_t scale_count);
 NSB_API int nsb_nvfp4_quantize(const nsb_matrix* value, int32_t transpose, const nsb_nvfp4* out,
-                               void* workspace, size_t workspace_bytes, void* stream);
+                               float* amax, int32_t amax_given, void* workspace,
+                               size_t workspace_bytes, void* stream);
 NSB_API int nsb_nvfp4_dequantize(const nsb_nvfp4* value, const nsb_matrix* out, void* stream);
 
 /* out[m, n] = sum over k of a[m, k] b[n, k], plus bias[n] where bias is given (float32).  Sums are

@@ -101,8 +101,8 @@ size_t nsb_nvfp4_quantize_workspace_size(int64_t rows, int64_t cols, int32_t tra
   return nsb::nvfp4_quantize_workspace_bytes(out, transpose != 0);
 }
 
-int nsb_nvfp4_quantize(const nsb_matrix* value, int32_t transpose, const nsb_nvfp4* out, void* workspace,
-                       size_t workspace_bytes, void* stream) {
+int nsb_nvfp4_quantize(const nsb_matrix* value, int32_t transpose, const nsb_nvfp4* out, float* amax,
+                       int32_t amax_given, void* workspace, size_t workspace_bytes, void* stream) {
   nsb::Dense v;
   nsb::Nvfp4 o;
   if (!check_matrix(value, &v, "the value must be a matrix of float32, float16 or bfloat16", "the value is required") ||
@@ -110,11 +110,13 @@ int nsb_nvfp4_quantize(const nsb_matrix* value, int32_t transpose, const nsb_nvf
     return NSB_ERR_ARGUMENT;
   if (o.rows != (transpose ? v.cols : v.rows) || o.cols != (transpose ? v.rows : v.cols))
     return nsb::set_error(NSB_ERR_ARGUMENT, "the NVFP4 matrix must have the value's shape, or the transposed one");
+  if (reinterpret_cast<uintptr_t>(amax) % 4 != 0 || (amax_given && !amax))
+    return nsb::set_error(NSB_ERR_ARGUMENT, "a given amax is required, 4-byte aligned");
   const size_t need = nsb_nvfp4_quantize_workspace_size(v.rows, v.cols, transpose, out->scale_count);
   if (!check_workspace(workspace, workspace_bytes, need, 4)) return NSB_ERR_WORKSPACE;
   nsb::set_error(NSB_OK, "");
   if (v.rows == 0) return NSB_OK;
-  return done(nsb::launch_nvfp4_quantize(v, transpose != 0, o, workspace, static_cast<cudaStream_t>(stream)),
+  return done(nsb::launch_nvfp4_quantize(v, transpose != 0, o, reinterpret_cast<unsigned int*>(amax), amax_given != 0, workspace, static_cast<cudaStream_t>(stream)),
               "nsb_nvfp4_quantize launch");
 }
 

@@ -28,8 +28,8 @@ struct Nvfp4 {
   bool per_row;
 };
 size_t nvfp4_quantize_workspace_bytes(const Nvfp4& out, bool transpose);
-cudaError_t launch_nvfp4_quantize(const Dense& value, bool transpose, const Nvfp4& out,
-                                  void* workspace, cudaStream_t stream);
+cudaError_t launch_nvfp4_quantize(const Dense& value, bool transpose, const Nvfp4& out, unsigned int* amax,
+                                  bool amax_given, void* workspace, cudaStream_t stream);
 cudaError_t launch_nvfp4_dequantize(const Nvfp4& in, const Dense& out, cudaStream_t stream);
 size_t column_sums_workspace_bytes(int64_t rows, int64_t cols);
 cudaError_t launch_column_sums(const Dense& value, float* out, void* workspace, cudaStream_t stream);

@@ -93,25 +93,31 @@ def quantize_nvfp4(value: torch.Tensor, *, per: str = "row", transpose: bool = F
     """
     if per not in ("row", "tensor"):
         raise ValueError("per must be 'row' or 'tensor'")
-    value = value.detach()
+    return _quantize(value.detach(), per == "row", transpose)
+
+
+def _quantize(value: torch.Tensor, per_row: bool, transpose: bool, amax: torch.Tensor | None = None,
+              given: bool = False) -> Nvfp4Matrix:
+    """``amax``: a float32 word that receives the largest |value|, or (``given``) holds it already."""
     view = dense_matrix(value, "value")
-    rows, columns = (value.shape[1], value.shape[0]) if transpose else value.shape
-    if value.shape[1] < 1 or columns < 1:
+    rows, columns = (view.cols, view.rows) if transpose else (view.rows, view.cols)
+    if view.cols < 1 or columns < 1:
         raise ValueError("an NVFP4 matrix needs at least one column")
     device = value.device
     codes = torch.empty((rows, (columns + 31) // 32 * 16), device=device, dtype=torch.uint8)
     scales = torch.empty(((rows + 127) // 128, (columns + 255) // 256 * 4, 512), device=device,
                          dtype=torch.uint8)
     # A tensor without rows has the scale of zeros.
-    scale = (torch.empty if rows else torch.ones)(rows if per == "row" else 1, device=device,
+    scale = (torch.empty if rows else torch.ones)(rows if per_row else 1, device=device,
                                                   dtype=torch.float32)
     packed = Nvfp4Matrix(codes, scales, scale, columns)
     lib = load_library()
     result = packed._view()
-    size = lib.nsb_nvfp4_quantize_workspace_size(*value.shape, int(transpose), scale.shape[0])
+    size = lib.nsb_nvfp4_quantize_workspace_size(view.rows, view.cols, int(transpose), scale.shape[0])
     workspace = torch.empty(size, device=device, dtype=torch.uint8) if size else None
     token_call(device, lib.nsb_nvfp4_quantize, ctypes.byref(view), int(transpose),
-               ctypes.byref(result), workspace.data_ptr() if size else None, size)
+               ctypes.byref(result), None if amax is None else amax.data_ptr(), int(given),
+               workspace.data_ptr() if size else None, size)
     return packed
 
 
@@ -177,24 +183,29 @@ class _Readout(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, state, weight, bias, dtype):
-        ctx.save_for_backward(state, weight)
-        return nvfp4_product(quantize_nvfp4(state), quantize_nvfp4(weight, per="tensor"),
+        # The largest sizes of state and weight come with the forward's packing: the backward's needs no pass for them.
+        most = torch.empty(2, device=state.device, dtype=torch.float32)
+        ctx.save_for_backward(state, weight, most)
+        return nvfp4_product(_quantize(state, True, False, most[:1]), _quantize(weight, False, False, most[1:]),
                              bias=None if bias is None else bias.detach(), dtype=dtype)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        state, weight = ctx.saved_tensors
+        state, weight, most = ctx.saved_tensors
         dx = dw = db = None
         if grad.stride(1) != 1 and grad.shape[1] > 1 or grad.shape[0] > 1 and grad.stride(0) < grad.shape[1]:
             grad = grad.contiguous()  # e.g. the expanded gradient of a sum
+        grad_most = None
         if ctx.needs_input_grad[0]:
-            dx = nvfp4_product(quantize_nvfp4(grad), quantize_nvfp4(weight, per="tensor", transpose=True),
+            if ctx.needs_input_grad[1]:
+                grad_most = torch.empty(1, device=grad.device, dtype=torch.float32)
+            dx = nvfp4_product(_quantize(grad, True, False, grad_most), _quantize(weight, False, True, most[1:], True),
                                dtype=state.dtype)
         if ctx.needs_input_grad[1]:
             if state.shape[0]:
-                dw = nvfp4_product(quantize_nvfp4(grad, per="tensor", transpose=True),
-                                   quantize_nvfp4(state, per="tensor", transpose=True), dtype=weight.dtype)
+                dw = nvfp4_product(_quantize(grad, False, True, grad_most, grad_most is not None),
+                                   _quantize(state, False, True, most[:1], True), dtype=weight.dtype)
             else:
                 dw = torch.zeros_like(weight)
         if ctx.needs_input_grad[2]:

@@ -265,7 +265,7 @@ def load_library() -> ctypes.CDLL:
                                           size, ptr]
     lib.nsb_nvfp4_quantize_workspace_size.argtypes = [i64, i64, i32, i64]
     lib.nsb_nvfp4_quantize_workspace_size.restype = size
-    lib.nsb_nvfp4_quantize.argtypes = [p(_Matrix), i32, p(_Nvfp4), ptr, size, ptr]
+    lib.nsb_nvfp4_quantize.argtypes = [p(_Matrix), i32, p(_Nvfp4), ptr, i32, ptr, size, ptr]
     lib.nsb_nvfp4_dequantize.argtypes = [p(_Nvfp4), p(_Matrix), ptr]
     lib.nsb_nvfp4_product.argtypes = [p(_Nvfp4), p(_Nvfp4), ptr, p(_Matrix), ptr, ptr]
     lib.nsb_column_sums_workspace_size.argtypes = [i64, i64]

@@ -93,14 +93,14 @@ def test_entry_points_refuse_bad_arguments():
     def packed(rows=4, cols=40, codes=p, stride=32, scales=p, scale=p, count=1):
         return native._Nvfp4(rows, cols, codes, stride, scales, scale, count)
 
-    def quantize(value=value, transpose=0, out=None, workspace=p, size=4):
-        return lib.nsb_nvfp4_quantize(ctypes.byref(value), transpose, ctypes.byref(out or packed()), workspace, size, None)
+    def quantize(value=value, transpose=0, out=None, workspace=p, size=4, given=0):
+        return lib.nsb_nvfp4_quantize(ctypes.byref(value), transpose, ctypes.byref(out or packed()), None, given, workspace, size, None)
 
     for bad in (packed(rows=5), packed(cols=41), packed(stride=16), packed(codes=p + 8), packed(scales=None),
                 packed(scale=p + 2), packed(count=3), packed(codes=None), packed(rows=-1), packed(cols=0, stride=0)):
         assert quantize(out=bad) == -1
         assert lib.nsb_last_error()
-    assert quantize(transpose=1) == -1 and quantize(value=native._Matrix(p, 4, 40, 40, 7)) == -1
+    assert quantize(given=1) == -1 and quantize(transpose=1) == -1 and quantize(value=native._Matrix(p, 4, 40, 40, 7)) == -1
     assert quantize(workspace=None) == -3 and quantize(size=3) == -3 and quantize(workspace=p + 2) == -3
     out = native._Matrix(p, 4, 6, 6, 0)
 
