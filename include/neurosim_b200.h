@@ -634,7 +634,7 @@ typedef struct nsb_row_values {
  * of the row's largest out value, -1 where none is above -inf (NaN is never chosen).  Lengths are
  * clamped to [0, history_length]; history entries outside [0, vocabulary) are skipped. */
 typedef struct nsb_logits {
-  nsb_matrix logits, out;  /* [rows, vocabulary], same type; out may be the logits themselves */
+  nsb_matrix logits, out;  /* [rows, vocabulary < 2^30], same type; out may be the logits themselves */
   const int32_t* history;  /* [rows, history_length] */
   int64_t history_length, history_stride;
   const int32_t* lengths;        /* [rows], NULL: history_length */

@@ -173,6 +173,7 @@ int nsb_adjust_logits(const nsb_logits* args, void* stream) {
     return NSB_ERR_ARGUMENT;
   if (a.out.rows != a.logits.rows || a.out.cols != a.logits.cols || a.out.type != a.logits.type)
     return nsb::set_error(NSB_ERR_ARGUMENT, "the output must have the logits' shape and type");
+  if (a.logits.cols >= kMost / 2) return nsb::set_error(NSB_ERR_ARGUMENT, "the vocabulary must be below 2^30");
   if (args->history_length < 0 || args->history_length >= kMost || (args->history_length > 0 && a.logits.rows > 0 && (!args->history || args->history_stride < 0)))
     return nsb::set_error(NSB_ERR_ARGUMENT, "the history must be [rows, length] int32");
   if ((args->bias && args->bias_stride < 0) || (args->mask && args->mask_stride < 0) ||

@@ -387,22 +387,22 @@ dequantize_kernel(Nvfp4 in, Dense out, unsigned chunks) {
     if (!valid) return;
     float level[8];
     e2m1_levels8(codes, level);
-    O v[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = Values<O>::down(__fmul_rn(level[k], step));
+    for (int k = 0; k < 8; ++k) level[k] = __fmul_rn(level[k], step);
+    const Pack<O, 8> v = round_pack<O, 8>(level);
     O* to = static_cast<O*>(out.data) + r * out.stride + c;
     if (c + 8 <= in.cols) {
 #pragma unroll
       for (int q = 0; q < 8 / P; ++q) {
         Pack<O, P> x;
 #pragma unroll
-        for (int k = 0; k < P; ++k) x.v[k] = v[q * P + k];
+        for (int k = 0; k < P; ++k) x.v[k] = v.v[q * P + k];
         store_pack<O, P>(to + q * P, x);
       }
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        if (c + k < in.cols) to[k] = v[k];
+        if (c + k < in.cols) to[k] = v.v[k];
     }
   } else {  // blockDim.x is a multiple of 32: a warp holds one row
     if (r >= in.rows) return;

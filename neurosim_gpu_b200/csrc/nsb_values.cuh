@@ -29,12 +29,14 @@ struct Values<float> {
 };
 template <>
 struct Values<__half> {
+  using Two = __half2;
   static constexpr int kType = NSB_VALUE_F16;
   __device__ static __forceinline__ float up(__half v) { return __half2float(v); }
   __device__ static __forceinline__ __half down(float v) { return __float2half_rn(v); }
 };
 template <>
 struct Values<__nv_bfloat16> {
+  using Two = __nv_bfloat162;
   static constexpr int kType = NSB_VALUE_BF16;
   __device__ static __forceinline__ float up(__nv_bfloat16 v) { return __bfloat162float(v); }
   __device__ static __forceinline__ __nv_bfloat16 down(float v) { return __float2bfloat16_rn(v); }
@@ -54,6 +56,31 @@ __device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
 template <typename T, int V>
 __device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& v) {
   *reinterpret_cast<Pack<T, V>*>(p) = v;
+}
+
+// V float32 values rounded to T.  Two at a time: the conversion of a single value to 16 bits runs on the
+// slow special-function pipe, that of a pair does not.
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> round_pack(const float (&v)[V]) {
+  Pack<T, V> r;
+  if constexpr (sizeof(T) == 4 || V == 1) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.v[i] = Values<T>::down(v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      if constexpr (Values<T>::kType == NSB_VALUE_BF16) {
+        const __nv_bfloat162 x = __floats2bfloat162_rn(v[i], v[i + 1]);
+        r.v[i] = x.x;
+        r.v[i + 1] = x.y;
+      } else {
+        const __half2 x = __floats2half2_rn(v[i], v[i + 1]);
+        r.v[i] = x.x;
+        r.v[i + 1] = x.y;
+      }
+    }
+  }
+  return r;
 }
 
 // Whether every row of `m` starts on a multiple of `bytes`.

@@ -60,8 +60,10 @@ drive_kernel(const void* tokens, int token_bytes, int64_t n, Dense table, float 
   Pack<O, V> r;
   if (token >= 0 && token < table.rows) {
     const Pack<In, V> x = load_pack<In, V>(static_cast<const In*>(table.data) + token * table.stride + c);
+    float y[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) r.v[i] = Values<O>::down(__fmul_rn(Values<In>::up(x.v[i]), scale));
+    for (int i = 0; i < V; ++i) y[i] = __fmul_rn(Values<In>::up(x.v[i]), scale);
+    r = round_pack<O, V>(y);
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i) r.v[i] = Values<O>::down(0.0f);
@@ -221,10 +223,10 @@ segment_kernel(const uint32_t* __restrict__ key, const uint32_t* __restrict__ po
   auto flush = [&](bool tail) {
     if (run >= limit) return;
     if (!head && !tail) {
-      Pack<O, V> r;
+      float r[V];
 #pragma unroll
-      for (int v = 0; v < V; ++v) r.v[v] = Values<O>::down(__fmul_rn(acc[v], scale));
-      store_pack<O, V>(static_cast<O*>(out.data) + run * out.stride + c, r);
+      for (int v = 0; v < V; ++v) r[v] = __fmul_rn(acc[v], scale);
+      store_pack<O, V>(static_cast<O*>(out.data) + run * out.stride + c, round_pack<O, V>(r));
     } else {
       float* to = partials.row(j, head ? 0 : 1) + c;
 #pragma unroll

@@ -142,7 +142,8 @@ def test_function_refuses_bad_arguments():
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,vocabulary,length", [(0, 5, 3), (1, 1, 0), (1, 1, 4), (2, 31, 1), (1, 33, 17), (3, 1000, 0),
-                                                    (5, 4097, 300), (2, 70_001, 5000), (1, 131_072, 64)])
+                                                    (5, 4097, 300), (2, 70_001, 5000), (1, 131_072, 64), (2, 200_003, 40_000),
+                                                    (1, 600_000, 5000), (700, 130, 9)])
 def test_adjust(dtype, rows, vocabulary, length):
     logits = (3 * torch.randn(rows, vocabulary, generator=generator(1))).to(dtype)
     check(logits, dtype, **case(rows, vocabulary, length))
