@@ -21,6 +21,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "nsb_tokens.h"
 
@@ -34,8 +35,10 @@ constexpr int kSortCtas = 8;       // one portable cluster
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kDigits = 256;
+constexpr int kHeld = 8;           // of a warp's rounds in registers: 65,536 tokens in all
 constexpr int kSegmentThreads = 128;
-constexpr int kJoinGroups = 16;
+constexpr int kTileMost = 64;
+constexpr int kJoinWarps = 8;
 
 __device__ __forceinline__ int64_t token_at(const void* tokens, int bytes, int64_t t) {
   return bytes == 8 ? __ldg(static_cast<const long long*>(tokens) + t)
@@ -46,29 +49,73 @@ __device__ __forceinline__ int64_t token_at(const void* tokens, int bytes, int64
 // Drive
 // ---------------------------------------------------------------------------
 
-// blockDim = (vectors of a row, rows of the block); the grid runs over row groups x column chunks.
-template <typename In, typename O, int V>
-__global__ void __launch_bounds__(kDriveThreads)
-drive_kernel(const void* tokens, int token_bytes, int64_t n, Dense table, float scale, Dense out,
-             int64_t chunks) {
-  const int64_t group = blockIdx.x / chunks;
-  const int64_t t = group * blockDim.y + threadIdx.y;
-  const int64_t c = ((blockIdx.x - group * chunks) * blockDim.x + threadIdx.x) * V;
-  if (t >= n || c >= out.cols) return;
-  const int64_t token = token_at(tokens, token_bytes, t);
-  O* to = static_cast<O*>(out.data) + t * out.stride + c;
-  Pack<O, V> r;
-  if (token >= 0 && token < table.rows) {
-    const Pack<In, V> x = load_pack<In, V>(static_cast<const In*>(table.data) + token * table.stride + c);
-    float y[V];
+// 16 bytes of values from any place p.  Off a 16-byte boundary they are cut out of the two aligned
+// vectors around them, as long as these lie within [first, last); p + 16 bytes does.
+template <typename T>
+__device__ __forceinline__ Pack<T, 16 / sizeof(T)> load_anywhere(const T* p, const T* first, const T* last) {
+  constexpr int P = 16 / static_cast<int>(sizeof(T));
+  const int lead = static_cast<int>(reinterpret_cast<uintptr_t>(p) % 16 / sizeof(T));
+  if (lead == 0) return load_pack<T, P>(p);
+  Pack<T, P> r;
+  const T* from = p - lead;
+  if (from >= first && from + 2 * P <= last) {
+    const uint4 a = *reinterpret_cast<const uint4*>(from), b = *(reinterpret_cast<const uint4*>(from) + 1);
+    const uint32_t all[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    const int words = lead * static_cast<int>(sizeof(T)) / 4, bits = lead * static_cast<int>(sizeof(T)) % 4 * 8;
+    auto* to = reinterpret_cast<uint32_t*>(&r);
+    auto cut = [&](auto skip) {
+      constexpr int kSkip = decltype(skip)::value;
 #pragma unroll
-    for (int i = 0; i < V; ++i) y[i] = __fmul_rn(Values<In>::up(x.v[i]), scale);
-    r = round_pack<O, V>(y);
+      for (int i = 0; i < 4; ++i) to[i] = __funnelshift_r(all[i + kSkip], all[(i + kSkip + 1) % 8], bits);
+    };
+    if (words == 0) cut(std::integral_constant<int, 0>{});
+    else if (words == 1) cut(std::integral_constant<int, 1>{});
+    else if (words == 2) cut(std::integral_constant<int, 2>{});
+    else cut(std::integral_constant<int, 3>{});
   } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) r.v[i] = Values<O>::down(0.0f);
+    for (int i = 0; i < P; ++i) r.v[i] = p[i];
   }
-  store_pack<O, V>(to, r);
+  return r;
+}
+
+// blockDim = (vectors of a row, rows of the block); the grid runs over row groups x column chunks.  A
+// vector is 16 bytes of the table's type.  kAligned: rows of both matrices start on vectors; else a row
+// is cut where its output reaches a vector's boundary, and the table's values are shifted into place
+// (4,000 x 4,001 bf16: 14.4 us; single columns a warp's width apart 20.0; on vectors 6 would do).
+template <typename In, typename O, bool kAligned>
+__global__ void __launch_bounds__(kDriveThreads)
+drive_kernel(const void* tokens, int token_bytes, int64_t n, Dense table, float scale, Dense out,
+             unsigned chunks) {
+  constexpr int V = 16 / static_cast<int>(sizeof(In));
+  const unsigned group = blockIdx.x / chunks;
+  const int64_t t = static_cast<int64_t>(group) * blockDim.y + threadIdx.y;
+  if (t >= n) return;
+  O* row = static_cast<O*>(out.data) + t * out.stride;
+  const int shift = kAligned ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(row) % (V * sizeof(O)) / sizeof(O));
+  const int64_t c = static_cast<int64_t>((blockIdx.x - group * chunks) * blockDim.x + threadIdx.x) * V - shift;
+  if (c >= out.cols) return;
+  const int64_t token = token_at(tokens, token_bytes, t);
+  const bool valid = token >= 0 && token < table.rows;
+  const In* first = static_cast<const In*>(table.data);
+  const In* from = first + (valid ? token : 0) * table.stride;
+  if (c >= 0 && c + V <= out.cols) {
+    float y[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) y[i] = 0.0f;
+    if (valid) {
+      Pack<In, V> x;
+      if constexpr (kAligned) x = load_pack<In, V>(from + c);
+      else x = load_anywhere<In>(from + c, first, first + (table.rows - 1) * table.stride + table.cols);
+#pragma unroll
+      for (int i = 0; i < V; ++i) y[i] = __fmul_rn(Values<In>::up(x.v[i]), scale);
+    }
+    store_pack<O, V>(row + c, round_pack<O, V>(y));
+  } else {
+    for (int i = 0; i < V; ++i)
+      if (c + i >= 0 && c + i < out.cols)
+        row[c + i] = Values<O>::down(valid ? __fmul_rn(Values<In>::up(from[c + i]), scale) : 0.0f);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -87,7 +134,7 @@ struct Sorted {
 // its digits; the warp walks its elements again in order and places them.
 __device__ void sort_tokens(cg::cluster_group& cluster, const void* tokens, int token_bytes,
                             int64_t n, int64_t limit, const Sorted& s, int passes,
-                            uint32_t (*hist)[kDigits], uint32_t* totals, uint32_t* scan) {
+                            uint32_t (*hist)[kDigits], uint32_t* totals, uint32_t* scan, uint32_t* first_of) {
   const int rank = static_cast<int>(cluster.block_rank());
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t span = ((n + kSortCtas * kSortWarps - 1) / (kSortCtas * kSortWarps) + 31) / 32 * 32;
@@ -102,32 +149,50 @@ __device__ void sort_tokens(cg::cluster_group& cluster, const void* tokens, int 
       const int64_t token = token_at(tokens, token_bytes, i);
       return static_cast<uint32_t>(token < 0 || token >= limit ? limit : token);
     };
+    auto pos_of = [&](int64_t i) { return pass > 0 ? __ldcg(s.pos[(pass - 1) & 1] + i) : static_cast<uint32_t>(i); };
+    // The first kHeld rounds of 32 elements stay in registers for both walks.
+    uint32_t held[kHeld], held_pos[kHeld];
+#pragma unroll
+    for (int r = 0; r < kHeld; ++r) {
+      const int64_t i = first + 32 * r + lane;
+      held[r] = i < last ? key_of(i) : 0;
+      held_pos[r] = i < last ? pos_of(i) : 0;
+    }
     for (int d = lane; d < kDigits; d += 32) hist[warp][d] = 0;
     __syncwarp();
-    for (int64_t i = first; i < last; i += 32) {
-      const bool in = i + lane < last;
-      const uint32_t digit = in ? (key_of(i + lane) >> shift) & (kDigits - 1) : ~0u;
+    auto count = [&](int64_t i, uint32_t key) {
+      const bool in = i < last;
+      const uint32_t digit = in ? (key >> shift) & (kDigits - 1) : ~0u;
       const uint32_t same = __match_any_sync(0xffffffffu, digit);
       if (in && (same & below) == 0) hist[warp][digit] += __popc(same);
       __syncwarp();
-    }
+    };
+#pragma unroll
+    for (int r = 0; r < kHeld; ++r)
+      if (first + 32 * r < last) count(first + 32 * r + lane, held[r]);
+    for (int64_t i = first + 32 * kHeld; i < last; i += 32) count(i + lane, i + lane < last ? key_of(i + lane) : 0);
     __syncthreads();
     if (threadIdx.x < kDigits) {
-      uint32_t sum = 0;
+      uint32_t c[kSortWarps], sum = 0;
+#pragma unroll
+      for (int w = 0; w < kSortWarps; ++w) c[w] = hist[w][threadIdx.x];
+#pragma unroll
       for (int w = 0; w < kSortWarps; ++w) {
-        const uint32_t c = hist[w][threadIdx.x];
         hist[w][threadIdx.x] = sum;
-        sum += c;
+        sum += c[w];
       }
       totals[threadIdx.x] = sum;
     }
     cluster.sync();
     uint32_t before = 0, all = 0;
     if (threadIdx.x < kDigits) {
+      uint32_t x[kSortCtas];
+#pragma unroll
+      for (int c = 0; c < kSortCtas; ++c) x[c] = *cluster.map_shared_rank(totals + threadIdx.x, c);
+#pragma unroll
       for (int c = 0; c < kSortCtas; ++c) {
-        const uint32_t x = *cluster.map_shared_rank(totals + threadIdx.x, c);
-        before += c < rank ? x : 0;
-        all += x;
+        before += c < rank ? x[c] : 0;
+        all += x[c];
       }
       // Exclusive scan over the digits: within the warp, then over the 8 warps that hold them.
       uint32_t sum = all;
@@ -142,20 +207,17 @@ __device__ void sort_tokens(cg::cluster_group& cluster, const void* tokens, int 
     if (threadIdx.x < kDigits) {
       uint32_t base = before + all;
       for (int w = 0; w < warp; ++w) base += scan[w];
-      for (int w = 0; w < kSortWarps; ++w) hist[w][threadIdx.x] += base;
+      first_of[threadIdx.x] = base;
     }
     __syncthreads();
     uint32_t* key_out = s.key[pass & 1];
     uint32_t* pos_out = s.pos[pass & 1];
-    for (int64_t i = first; i < last; i += 32) {
-      const bool in = i + lane < last;
-      const uint32_t key = in ? key_of(i + lane) : 0;
-      const uint32_t pos = !in ? 0 : pass > 0 ? __ldcg(s.pos[(pass - 1) & 1] + i + lane)
-                                              : static_cast<uint32_t>(i + lane);
+    auto place = [&](int64_t i, uint32_t key, uint32_t pos) {
+      const bool in = i < last;
       const uint32_t digit = in ? (key >> shift) & (kDigits - 1) : ~0u;
       const uint32_t same = __match_any_sync(0xffffffffu, digit);
       uint32_t slot = 0;
-      if (in) slot = hist[warp][digit] + __popc(same & below);
+      if (in) slot = first_of[digit] + hist[warp][digit] + __popc(same & below);
       __syncwarp();
       if (in && (same & below) == 0) hist[warp][digit] += __popc(same);
       __syncwarp();
@@ -163,36 +225,42 @@ __device__ void sort_tokens(cg::cluster_group& cluster, const void* tokens, int 
         key_out[slot] = key;
         pos_out[slot] = pos;
       }
+    };
+#pragma unroll
+    for (int r = 0; r < kHeld; ++r)
+      if (first + 32 * r < last) place(first + 32 * r + lane, held[r], held_pos[r]);
+    for (int64_t i = first + 32 * kHeld; i < last; i += 32) {
+      const bool in = i + lane < last;
+      place(i + lane, in ? key_of(i + lane) : 0, in ? pos_of(i + lane) : 0);
     }
     cluster.sync();  // also orders this pass's keys in global memory before the next pass reads them
   }
 }
 
-template <typename O, int V>
 __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads)
-sort_fill_kernel(const void* tokens, int token_bytes, int64_t n, Sorted s, int passes, Dense out) {
+sort_fill_kernel(const void* tokens, int token_bytes, int64_t n, Sorted s, int passes, Dense out, int bytes_each) {
   __shared__ uint32_t hist[kSortWarps][kDigits];
   __shared__ uint32_t totals[kDigits];
   __shared__ uint32_t scan[kDigits / 32];
+  __shared__ uint32_t first_of[kDigits];
   cg::cluster_group cluster = cg::this_cluster();
   if (blockIdx.x < kSortCtas) {
-    sort_tokens(cluster, tokens, token_bytes, n, out.rows, s, passes, hist, totals, scan);
+    sort_tokens(cluster, tokens, token_bytes, n, out.rows, s, passes, hist, totals, scan, first_of);
     return;
   }
-  const int64_t vectors = out.cols / V;  // V divides the columns
-  const int64_t all = out.rows * vectors;
-  const int64_t stride = static_cast<int64_t>(gridDim.x - kSortCtas) * kSortThreads;
-  Pack<O, V> zero;
-#pragma unroll
-  for (int i = 0; i < V; ++i) zero.v[i] = Values<O>::down(0.0f);
-  int64_t i = static_cast<int64_t>(blockIdx.x - kSortCtas) * kSortThreads + threadIdx.x;
-  if (out.stride == out.cols) {
-    for (; i < all; i += stride) store_pack<O, V>(static_cast<O*>(out.data) + i * V, zero);
-  } else {
-    for (; i < all; i += stride) {
-      const int64_t row = i / vectors;
-      store_pack<O, V>(static_cast<O*>(out.data) + row * out.stride + (i - row * vectors) * V, zero);
-    }
+  // Zero is all bits clear in every type.  The CTAs share the 16-byte vectors of contiguous rows, or take
+  // a row each.
+  const bool whole = out.stride == out.cols;
+  const int64_t ctas = gridDim.x - kSortCtas, cta = blockIdx.x - kSortCtas;
+  const int64_t bytes = (whole ? out.rows : 1) * out.cols * bytes_each;
+  const int64_t stride = (whole ? ctas : 1) * kSortThreads, own = (whole ? cta : 0) * kSortThreads + threadIdx.x;
+  for (int64_t r = whole ? 0 : cta; r < (whole ? 1 : out.rows); r += ctas) {
+    uint8_t* row = static_cast<uint8_t*>(out.data) + r * out.stride * bytes_each;
+    const int64_t head = min(bytes, static_cast<int64_t>((16 - reinterpret_cast<uintptr_t>(row) % 16) % 16));
+    const int64_t vectors = (bytes - head) / 16;
+    for (int64_t i = own; i < vectors; i += stride) reinterpret_cast<uint4*>(row + head)[i] = make_uint4(0, 0, 0, 0);
+    if (own < head) row[own] = 0;
+    if (own < bytes - head - vectors * 16) row[head + vectors * 16 + own] = 0;
   }
 }
 
@@ -205,18 +273,31 @@ struct Partials {
   }
 };
 
-template <typename In, typename O, int V>
-__global__ void __launch_bounds__(kSegmentThreads)
+// A thread sums 16 bytes' worth of columns: a vector (kAligned: rows of both matrices start on vectors),
+// or single columns kSegmentThreads apart (60,000 tokens x 1,001 bf16: 40 us; cutting vectors out of
+// aligned loads 95: too many selects in front of the sums).
+template <typename In, typename O, bool kAligned>
+__global__ void __launch_bounds__(kSegmentThreads, kAligned ? 8 : 6)
 segment_kernel(const uint32_t* __restrict__ key, const uint32_t* __restrict__ pos, int64_t n,
                int tile, Dense grad, float scale, Dense out, Partials partials, int slices) {
-  constexpr int U = 8;  // rows in flight per thread
+  constexpr int U = kAligned ? 8 : 4;  // rows in flight per thread
+  constexpr int V = 16 / static_cast<int>(sizeof(In));
+  __shared__ uint32_t keys[kTileMost + 2], places[kTileMost];  // keys: with the neighbours of the tile
   const int64_t j = blockIdx.x / slices;
-  const int64_t c = (static_cast<int64_t>(blockIdx.x - j * slices) * kSegmentThreads + threadIdx.x) * V;
+  constexpr int kStep = kAligned ? 1 : kSegmentThreads;  // between a thread's columns
+  const int64_t c = static_cast<int64_t>(blockIdx.x - j * slices) * kSegmentThreads * V + (kAligned ? threadIdx.x * V : threadIdx.x);
+  const int64_t i0 = j * tile;
+  const int count = static_cast<int>(min(n - i0, static_cast<int64_t>(tile)));
+  if (threadIdx.x < count + 2) {
+    const int64_t i = i0 + threadIdx.x - 1;
+    keys[threadIdx.x] = i >= 0 && i < n ? __ldg(key + i) : ~0u;  // beyond the ends: no token's key
+  }
+  if (threadIdx.x < count) places[threadIdx.x] = __ldg(pos + i0 + threadIdx.x);
+  __syncthreads();
   if (c >= grad.cols) return;
-  const int64_t i0 = j * tile, i1 = min(n, i0 + tile);
   const uint32_t limit = static_cast<uint32_t>(out.rows);
-  uint32_t run = __ldg(key + i0);
-  bool head = i0 > 0 && __ldg(key + i0 - 1) == run;
+  uint32_t run = keys[1];
+  bool head = keys[0] == run;
   float acc[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) acc[v] = 0.0f;
@@ -226,58 +307,63 @@ segment_kernel(const uint32_t* __restrict__ key, const uint32_t* __restrict__ po
       float r[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) r[v] = __fmul_rn(acc[v], scale);
-      store_pack<O, V>(static_cast<O*>(out.data) + run * out.stride + c, round_pack<O, V>(r));
+      O* to = static_cast<O*>(out.data) + run * out.stride + c;
+      if constexpr (kAligned) {
+        store_pack<O, V>(to, round_pack<O, V>(r));
+      } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+          if (c + v * kStep < out.cols) to[v * kStep] = Values<O>::down(r[v]);
+      }
     } else {
       float* to = partials.row(j, head ? 0 : 1) + c;
 #pragma unroll
-      for (int v = 0; v < V; ++v) to[v] = acc[v];
+      for (int v = 0; v < V; ++v)
+        if (kAligned || c + v * kStep < out.cols) to[v * kStep] = acc[v];
     }
   };
-  for (int64_t i = i0; i < i1; i += U) {
-    uint32_t k[U];
+  for (int i = 0; i < count; i += U) {
     Pack<In, V> g[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      k[u] = i + u < i1 ? __ldg(key + i + u) : limit;
-      const uint32_t p = i + u < i1 ? __ldg(pos + i + u) : 0;
-      if (k[u] < limit) {
-        g[u] = load_pack<In, V>(static_cast<const In*>(grad.data) + p * grad.stride + c);
+    for (int u = 0; u < U; ++u) {  // a row again where the tile ends
+      const In* from = static_cast<const In*>(grad.data) + places[min(i + u, count - 1)] * grad.stride + c;
+      if constexpr (kAligned) {
+        g[u] = load_pack<In, V>(from);
       } else {
 #pragma unroll
-        for (int v = 0; v < V; ++v) g[u].v[v] = Values<In>::down(0.0f);
+        for (int v = 0; v < V; ++v) g[u].v[v] = c + v * kStep < grad.cols ? from[v * kStep] : Values<In>::down(0.0f);
       }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (i + u < i1) {
-        if (k[u] != run) {
-          flush(false);
-          head = false;
-          run = k[u];
+      if (i + u >= count) break;
+      const uint32_t k = keys[1 + i + u];
+      if (k != run) {
+        flush(false);
+        head = false;
+        run = k;
 #pragma unroll
-          for (int v = 0; v < V; ++v) acc[v] = 0.0f;
-        }
-#pragma unroll
-        for (int v = 0; v < V; ++v) acc[v] += Values<In>::up(g[u].v[v]);
+        for (int v = 0; v < V; ++v) acc[v] = 0.0f;
       }
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[v] += Values<In>::up(g[u].v[v]);
     }
   }
-  flush(i1 < n && __ldg(key + i1) == run);
+  flush(keys[1 + count] == run);
 }
 
-// Tile j joins the run that starts in it and goes on into later tiles.  16 groups of 32 lanes
-// take every 16th tile of the run; their sums are added in group order.
+// Tile j joins the run that starts in it and goes on into later tiles.  A short run: each of the CTA's
+// warps takes 128 columns; a long one: the warps share its tiles, and their sums are added in warp order.
 template <typename O>
-__global__ void __launch_bounds__(32 * kJoinGroups)
+__global__ void __launch_bounds__(32 * kJoinWarps)
 join_kernel(const uint32_t* __restrict__ key, int64_t n, int tile, float scale, Dense out,
             Partials partials) {
-  __shared__ float4 sums[kJoinGroups][32];
+  __shared__ float4 sums[kJoinWarps][32];
   const int64_t j = blockIdx.x, i1 = (j + 1) * tile;
   if (i1 >= n) return;
-  const uint32_t run = __ldg(key + i1 - 1);
-  if (run >= static_cast<uint32_t>(out.rows) || __ldg(key + i1) != run) return;
-  if (j > 0 && __ldg(key + j * tile - 1) == run) return;  // the run started earlier
-  const int lane = threadIdx.x & 31, group = threadIdx.x >> 5;
+  const uint32_t run = __ldg(key + i1 - 1), after = __ldg(key + i1), ahead = j > 0 ? __ldg(key + j * tile - 1) : ~0u;
+  if (run >= static_cast<uint32_t>(out.rows) || after != run || ahead == run) return;  // ahead: it started earlier
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   // The last tile that the run reaches: 32 tiles' first keys at a time.
   int64_t last = j;
   for (;;) {
@@ -286,33 +372,48 @@ join_kernel(const uint32_t* __restrict__ key, int64_t n, int tile, float scale, 
     last += stop ? __ffs(stop) - 1 : 32;
     if (stop) break;
   }
+  const bool shared = last - j >= 128;
+  auto sum_of = [&](int64_t c, int64_t first, int step) {
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 16
+    for (int64_t t = first; t <= last; t += step) {
+      const float4 x = *reinterpret_cast<const float4*>(partials.row(t, t == j ? 1 : 0) + c);  // the pitch is a multiple of 8
+      sum.x += x.x;
+      sum.y += x.y;
+      sum.z += x.z;
+      sum.w += x.w;
+    }
+    return sum;
+  };
+  auto write = [&](int64_t c, const float4& sum) {
+    const float r[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+      if (c + v < out.cols)
+        static_cast<O*>(out.data)[run * out.stride + c + v] = Values<O>::down(__fmul_rn(r[v], scale));
+  };
+  if (!shared) {
+    for (int64_t c0 = (static_cast<int64_t>(blockIdx.y) * kJoinWarps + warp) * 128; c0 < out.cols; c0 += gridDim.y * kJoinWarps * 128) {
+      const int64_t c = c0 + 4 * lane;
+      if (c < out.cols) write(c, sum_of(c, j, 1));
+    }
+    return;
+  }
   for (int64_t c0 = static_cast<int64_t>(blockIdx.y) * 128; c0 < out.cols; c0 += gridDim.y * 128) {
     const int64_t c = c0 + 4 * lane;
-    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (c < out.cols) {  // the pitch is a multiple of 8: a float4 stays inside the row
-#pragma unroll 4
-      for (int64_t t = j + group; t <= last; t += kJoinGroups) {
-        const float4 x = *reinterpret_cast<const float4*>(partials.row(t, t == j ? 1 : 0) + c);
-        sum.x += x.x;
-        sum.y += x.y;
-        sum.z += x.z;
-        sum.w += x.w;
-      }
-    }
-    sums[group][lane] = sum;
+    sums[warp][lane] = c < out.cols ? sum_of(c, j + warp, kJoinWarps) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     __syncthreads();
-    if (group == 0) {
-      for (int g = 1; g < kJoinGroups; ++g) {
-        const float4 x = sums[g][lane];
+    if (warp == 0 && c < out.cols) {
+      float4 sum = sums[0][lane];
+#pragma unroll
+      for (int w = 1; w < kJoinWarps; ++w) {
+        const float4 x = sums[w][lane];
         sum.x += x.x;
         sum.y += x.y;
         sum.z += x.z;
         sum.w += x.w;
       }
-      const float r[4] = {sum.x, sum.y, sum.z, sum.w};
-      for (int v = 0; v < 4; ++v)
-        if (c + v < out.cols)
-          static_cast<O*>(out.data)[run * out.stride + c + v] = Values<O>::down(__fmul_rn(r[v], scale));
+      write(c, sum);
     }
     __syncthreads();
   }
@@ -320,29 +421,40 @@ join_kernel(const uint32_t* __restrict__ key, int64_t n, int tile, float scale, 
 
 int64_t partial_pitch(int64_t cols) { return (cols + 7) / 8 * 8; }
 
-// Long tiles leave fewer partials; short ones fill the GPU: about eight CTAs on each of 148 SMs.
+// Long tiles leave fewer partials; short ones fill the GPU: up to eight CTAs on each of 148 SMs.
 int64_t tile_of(int64_t n, int64_t slices) {
-  return std::max<int64_t>(8, std::min<int64_t>(64, n * slices / (148 * 8)));
+  return std::max<int64_t>(8, std::min<int64_t>(kTileMost, (n * slices + 148 * 8 - 1) / (148 * 8)));
 }
 
-template <typename In, typename O, int V>
+// Whether the rows of both matrices are whole vectors of 16 bytes of `In`.
+template <typename In, typename O>
+bool vectors_fit(const Dense& in, const Dense& out) {
+  constexpr int V = 16 / static_cast<int>(sizeof(In));
+  return out.cols % V == 0 && rows_aligned(in, sizeof(In), 16) && rows_aligned(out, sizeof(O), V * sizeof(O));
+}
+
+template <typename In, typename O>
 cudaError_t drive(const void* tokens, int token_bytes, int64_t n, const Dense& table, float scale,
                   const Dense& out, cudaStream_t stream) {
-  const int64_t vectors = (out.cols + V - 1) / V;
+  constexpr int V = 16 / static_cast<int>(sizeof(In));
+  const bool aligned = vectors_fit<In, O>(table, out);
+  const int64_t vectors = (out.cols + V - 1) / V + (aligned ? 0 : 1);
   int x = 32;
   while (x < kDriveThreads && x < vectors) x *= 2;
   const dim3 block(x, kDriveThreads / x);
   const int64_t chunks = (vectors + x - 1) / x;
   const int64_t groups = (n + block.y - 1) / block.y;
   if (chunks * groups > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  drive_kernel<In, O, V><<<static_cast<unsigned>(chunks * groups), block, 0, stream>>>(
-      tokens, token_bytes, n, table, scale, out, chunks);
+  auto* kernel = aligned ? drive_kernel<In, O, true> : drive_kernel<In, O, false>;
+  kernel<<<static_cast<unsigned>(chunks * groups), block, 0, stream>>>(tokens, token_bytes, n, table, scale, out,
+                                                                       static_cast<unsigned>(chunks));
   return cudaGetLastError();
 }
 
-template <typename In, typename O, int V>
+template <typename In, typename O>
 cudaError_t gradient(const void* tokens, int token_bytes, const Dense& grad, float scale,
                      const Dense& out, void* workspace, cudaStream_t stream) {
+  constexpr int V = 16 / static_cast<int>(sizeof(In));
   DeviceInfo info;
   cudaError_t err = device_info(&info);
   if (err != cudaSuccess) return err;
@@ -353,33 +465,24 @@ cudaError_t gradient(const void* tokens, int token_bytes, const Dense& grad, flo
   const Partials partials{reinterpret_cast<float*>(words + 4 * padded), partial_pitch(out.cols)};
   int passes = 1;
   while (passes < 4 && (out.rows >> (8 * passes)) > 0) ++passes;
-  const int64_t fill = (out.rows * (out.cols / V) + kSortThreads - 1) / kSortThreads;
-  const int64_t clusters = 1 + std::min<int64_t>((fill + kSortCtas - 1) / kSortCtas, info.sm_count / kSortCtas * 2);
-  sort_fill_kernel<O, V><<<static_cast<unsigned>(clusters * kSortCtas), kSortThreads, 0, stream>>>(
-      tokens, token_bytes, n, s, n > 0 ? passes : 0, out);
+  const int64_t fill = (out.rows * out.cols * static_cast<int64_t>(sizeof(O)) / 16 + kSortThreads - 1) / kSortThreads;
+  const int64_t clusters = 1 + std::min<int64_t>((fill + kSortCtas - 1) / kSortCtas + 1, info.sm_count / kSortCtas * 2);
+  sort_fill_kernel<<<static_cast<unsigned>(clusters * kSortCtas), kSortThreads, 0, stream>>>(
+      tokens, token_bytes, n, s, n > 0 ? passes : 0, out, static_cast<int>(sizeof(O)));
   if ((err = cudaGetLastError()) != cudaSuccess || n == 0) return err;
   const uint32_t* key = s.key[(passes - 1) & 1];
   const uint32_t* pos = s.pos[(passes - 1) & 1];
-  const int64_t slices = (out.cols / V + kSegmentThreads - 1) / kSegmentThreads;
+  const int64_t slices = (out.cols + V * kSegmentThreads - 1) / (V * kSegmentThreads);
   const int tile = static_cast<int>(tile_of(n, slices));
   const int64_t tiles = (n + tile - 1) / tile;
   if (tiles * slices > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  segment_kernel<In, O, V><<<static_cast<unsigned>(tiles * slices), kSegmentThreads, 0, stream>>>(
-      key, pos, n, tile, grad, scale, out, partials, static_cast<int>(slices));
+  auto* kernel = vectors_fit<In, O>(grad, out) ? segment_kernel<In, O, true> : segment_kernel<In, O, false>;
+  kernel<<<static_cast<unsigned>(tiles * slices), kSegmentThreads, 0, stream>>>(key, pos, n, tile, grad, scale, out, partials,
+                                                                                static_cast<int>(slices));
   if ((err = cudaGetLastError()) != cudaSuccess || tiles == 1) return err;
-  const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(std::min<int64_t>(8, (out.cols + 127) / 128)));
-  join_kernel<O><<<grid, 32 * kJoinGroups, 0, stream>>>(key, n, tile, scale, out, partials);
+  const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(std::min<int64_t>(16, std::max((out.cols + 1023) / 1024, std::min<int64_t>(4, (out.cols + 255) / 256)))));
+  join_kernel<O><<<grid, 32 * kJoinWarps, 0, stream>>>(key, n, tile, scale, out, partials);
   return cudaGetLastError();
-}
-
-// The widest vector, up to 16 bytes of `In`, that divides the columns and fits both matrices' rows.
-template <typename In, typename O>
-int vector_of(const Dense& in, const Dense& out) {
-  for (int v = 16 / static_cast<int>(sizeof(In)); v > 1; v /= 2)
-    if (out.cols % v == 0 && rows_aligned(in, sizeof(In), v * sizeof(In)) &&
-        rows_aligned(out, sizeof(O), v * sizeof(O)))
-      return v;
-  return 1;
 }
 
 }  // namespace
@@ -390,11 +493,7 @@ cudaError_t launch_stimulus_drive(const void* tokens, int token_bytes, int64_t n
     using In = decltype(in);
     auto call = [&](auto o) {
       using O = decltype(o);
-      const int v = vector_of<In, O>(table, out);
-      if (sizeof(In) == 2 && v == 8) return drive<In, O, sizeof(In) == 2 ? 8 : 4>(tokens, token_bytes, n, table, scale, out, stream);
-      if (v >= 4) return drive<In, O, 4>(tokens, token_bytes, n, table, scale, out, stream);
-      if (v == 2) return drive<In, O, 2>(tokens, token_bytes, n, table, scale, out, stream);
-      return drive<In, O, 1>(tokens, token_bytes, n, table, scale, out, stream);
+      return drive<In, O>(tokens, token_bytes, n, table, scale, out, stream);
     };
     return out.type == NSB_VALUE_F32 ? call(float{}) : call(in);
   });
@@ -414,11 +513,7 @@ cudaError_t launch_stimulus_gradient(const void* tokens, int token_bytes, const 
     using In = decltype(in);
     auto call = [&](auto o) {
       using O = decltype(o);
-      const int v = vector_of<In, O>(grad, out);
-      if (sizeof(In) == 2 && v == 8) return gradient<In, O, sizeof(In) == 2 ? 8 : 4>(tokens, token_bytes, grad, scale, out, workspace, stream);
-      if (v >= 4) return gradient<In, O, 4>(tokens, token_bytes, grad, scale, out, workspace, stream);
-      if (v == 2) return gradient<In, O, 2>(tokens, token_bytes, grad, scale, out, workspace, stream);
-      return gradient<In, O, 1>(tokens, token_bytes, grad, scale, out, workspace, stream);
+      return gradient<In, O>(tokens, token_bytes, grad, scale, out, workspace, stream);
     };
     if constexpr (sizeof(In) == 4) return with_type(out.type, call);  // a wide drive of a narrow table
     return out.type == NSB_VALUE_F32 ? call(float{}) : call(in);
