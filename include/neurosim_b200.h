@@ -612,6 +612,14 @@ NSB_API int nsb_nvfp4_dequantize(const nsb_nvfp4* value, const nsb_matrix* out, 
 NSB_API int nsb_nvfp4_product(const nsb_nvfp4* a, const nsb_nvfp4* b, const float* bias,
                               const nsb_matrix* out, int* status, void* stream);
 
+/* States through packed weights: nsb_nvfp4_quantize of the states (a scale per row) into the workspace
+ * (16-byte aligned, contents need not be initialised), then nsb_nvfp4_product with the weights.  The
+ * product starts loading the weights while the states are packed. */
+NSB_API size_t nsb_nvfp4_readout_workspace_size(int64_t rows, int64_t cols);
+NSB_API int nsb_nvfp4_readout(const nsb_matrix* state, const nsb_nvfp4* weight, const float* bias,
+                              const nsb_matrix* out, void* workspace, size_t workspace_bytes,
+                              int* status, void* stream);
+
 /* out[c] = sum of column c of `value` (float32, in a fixed order): the gradient of a bias. */
 NSB_API size_t nsb_column_sums_workspace_size(int64_t rows, int64_t cols);
 NSB_API int nsb_column_sums(const nsb_matrix* value, float* out, void* workspace,

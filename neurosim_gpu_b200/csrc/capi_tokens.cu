@@ -145,8 +145,36 @@ int nsb_nvfp4_product(const nsb_nvfp4* a, const nsb_nvfp4* b, const float* bias,
   if (reinterpret_cast<uintptr_t>(bias) % 4 != 0) return nsb::set_error(NSB_ERR_ARGUMENT, "the bias must be 4-byte aligned");
   nsb::set_error(NSB_OK, "");
   if (x.rows == 0) return NSB_OK;
-  return done(nsb::launch_nvfp4_product(x, y, bias, o, status, static_cast<cudaStream_t>(stream)),
+  return done(nsb::launch_nvfp4_product(x, y, bias, o, false, status, static_cast<cudaStream_t>(stream)),
               "nsb_nvfp4_product launch");
+}
+
+size_t nsb_nvfp4_readout_workspace_size(int64_t rows, int64_t cols) {
+  if (rows < 1 || cols < 1 || rows >= kMost || cols >= kMost) return 0;
+  const int64_t codes = rows * ((cols + 31) / 32 * 16), scales = (rows + 127) / 128 * ((cols + 255) / 256) * 2048;
+  return static_cast<size_t>(codes + scales + 4 * rows);
+}
+
+int nsb_nvfp4_readout(const nsb_matrix* state, const nsb_nvfp4* weight, const float* bias, const nsb_matrix* out,
+                      void* workspace, size_t workspace_bytes, int* status, void* stream) {
+  nsb::Dense x, o;
+  nsb::Nvfp4 w;
+  if (!check_matrix(state, &x, "states must be a matrix of float32, float16 or bfloat16", "states are required") || !check_nvfp4(weight, &w) ||
+      !check_matrix(out, &o, "the output must be a matrix of float32, float16 or bfloat16", "the output is required"))
+    return NSB_ERR_ARGUMENT;
+  if (x.cols != w.cols) return nsb::set_error(NSB_ERR_ARGUMENT, "states and weights must have the same number of columns");
+  if (w.rows < 1 || o.rows != x.rows || o.cols != w.rows)
+    return nsb::set_error(NSB_ERR_ARGUMENT, "the output must be [state.rows, weight.rows], weight.rows >= 1");
+  if (reinterpret_cast<uintptr_t>(bias) % 4 != 0) return nsb::set_error(NSB_ERR_ARGUMENT, "the bias must be 4-byte aligned");
+  if (!check_workspace(workspace, workspace_bytes, nsb_nvfp4_readout_workspace_size(x.rows, x.cols), 16)) return NSB_ERR_WORKSPACE;
+  nsb::set_error(NSB_OK, "");
+  if (x.rows == 0) return NSB_OK;
+  auto* bytes = static_cast<uint8_t*>(workspace);
+  const int64_t pitch = (x.cols + 31) / 32 * 16, scales = (x.rows + 127) / 128 * ((x.cols + 255) / 256) * 2048;
+  const nsb::Nvfp4 q{x.rows, x.cols, bytes, pitch, bytes + x.rows * pitch, reinterpret_cast<float*>(bytes + x.rows * pitch + scales), true};
+  const cudaError_t err = nsb::launch_nvfp4_quantize(x, false, q, nullptr, false, nullptr, static_cast<cudaStream_t>(stream));
+  if (err != cudaSuccess) return done(err, "nsb_nvfp4_readout launch");
+  return done(nsb::launch_nvfp4_product(q, w, bias, o, true, status, static_cast<cudaStream_t>(stream)), "nsb_nvfp4_readout launch");
 }
 
 size_t nsb_column_sums_workspace_size(int64_t rows, int64_t cols) {

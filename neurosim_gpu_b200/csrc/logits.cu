@@ -444,7 +444,8 @@ cudaError_t adjust_rows(const LogitsArgs& a, cudaStream_t stream) {
   // A counter, a logit and a place (below 2^16) for each token that may occur.
   constexpr int kEach = 4 + static_cast<int>(sizeof(T)) + 2;
   const int shared = room * kEach;
-  if ((err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kListed * kEach)) != cudaSuccess) return err;
+  static SharedLimit limits[2];
+  if (kHistory && (err = limits[threads == 256 ? 0 : 1].raise(kernel, kListed * kEach)) != cudaSuccess) return err;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(static_cast<unsigned>(a.logits.rows * ctas));
   config.blockDim = dim3(threads);

@@ -147,6 +147,7 @@ __global__ void __launch_bounds__(kRowThreads)
 quantize_rows_kernel(Dense x, Nvfp4 out, const unsigned int* given, unsigned int* most, int per_row, int cluster, unsigned work) {
   __shared__ unsigned int best_of[kRowThreads / 32];
   __shared__ unsigned int cta_best;
+  asm volatile("griddepcontrol.launch_dependents;");  // a product after it may start (and wait)
   if (blockIdx.x >= work) {  // zero scales for the rows that fill up the last 128
     const int64_t tiles = block_scale_tiles(x.cols);
     const int word = threadIdx.x & 127, row = (word & 3) * 32 + (word >> 2);

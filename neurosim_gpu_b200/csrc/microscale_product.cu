@@ -70,6 +70,7 @@ struct ProductArgs {
   int64_t scale_tiles;  // 512-byte tiles per 128 rows
   int32_t k_tiles, split;
   int32_t lane_tiles, column_tiles;
+  bool lane_ready;  // the operand along the lanes was complete before the kernel ahead of this one started
   int* status;
 };
 
@@ -153,8 +154,23 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
 
   if (warp == 0) {  // loads
     Ring<S::kStages> ring;
-    int n = 0;
+    int n = 0, ahead = 0;
     bool ok = true;
+    if (a.lane_ready && first < tiles) {  // its first stages' share while the kernel ahead still runs
+      int lt, ct;
+      place(a, first, &lt, &ct);
+      ahead = min(S::kStages, k1 - k0);
+      if (elect_one())
+        for (int s = 0; s < ahead; ++s) {
+          uint8_t* to = stages + s * S::kStageBytes;
+          barrier_arrive_expect(&h.full[s], S::kStageBytes);
+          load_box(to, &lane_map, (k0 + s) * kTileBytes, lt * kLanes, &h.full[s]);
+          load_bytes(to + kLaneBytes + kColumns * kTileBytes, a.lane.block_scales + (lt * a.scale_tiles + (k0 + s) * 4) * 512,
+                     kScaleBytes, &h.full[s]);
+        }
+      __syncwarp();
+    }
+    grid_wait();
     for (int tile = first; ok && tile < tiles; tile += step) {
       int lt, ct;
       place(a, tile, &lt, &ct);
@@ -174,11 +190,13 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
         }
         if (elect_one()) {
           uint8_t* to = stages + ring.stage * S::kStageBytes;
-          barrier_arrive_expect(full, S::kStageBytes);
-          load_box(to, &lane_map, k * kTileBytes, lt * kLanes, full);
+          if (n >= ahead) {
+            barrier_arrive_expect(full, S::kStageBytes);
+            load_box(to, &lane_map, k * kTileBytes, lt * kLanes, full);
+            load_bytes(to + kLaneBytes + kColumns * kTileBytes, lane_scales + k * kScaleBytes, kScaleBytes, full);
+          }
           load_box(to + kLaneBytes, &column_map, k * kTileBytes, ct * kColumns, full);
           to += kLaneBytes + kColumns * kTileBytes;
-          load_bytes(to, lane_scales + k * kScaleBytes, kScaleBytes, full);
 #pragma unroll
           for (int c = 0; c < S::kBlocks; ++c)
             load_bytes(to + kScaleBytes * (1 + c), column_scales[c] + k * kScaleBytes, kScaleBytes, full);
@@ -243,6 +261,7 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
       }
     }
   } else {  // results: a warp reads lanes 32 (warp % 4) ... of its columns
+    grid_wait();  // the scales may be the kernel's ahead, and what it reads may lie where this one writes
     const int quarter = warp & 3, slot = threadIdx.x - 64;
     const int part = (warp - 2) / 4 * S::kOutColumns;  // first column
     int t = 0;
@@ -380,25 +399,29 @@ cudaError_t launch(const Nvfp4& lane, const Nvfp4& column, ProductArgs a, int sm
   while (a.split < 8 && tiles * a.split * 2 <= sm_count && a.k_tiles >= a.split * 2) a.split *= 2;
   CUtensorMap lane_map, column_map;
   if (!map_codes(lane, kLanes, &lane_map) || !map_codes(column, kColumns, &column_map)) return cudaErrorInvalidValue;
-  const cudaError_t err = cudaFuncSetAttribute(product_kernel<O, kColumns>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kShared);
+  static SharedLimit limit;
+  const cudaError_t err = limit.raise(product_kernel<O, kColumns>, S::kShared);
   if (err != cudaSuccess) return err;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(static_cast<unsigned>(a.split > 1 ? tiles * a.split : std::min<int64_t>(tiles, sm_count)));
   config.blockDim = dim3(S::kThreads);
   config.dynamicSmemBytes = S::kShared;
   config.stream = stream;
-  cudaLaunchAttribute cluster{};
-  cluster.id = cudaLaunchAttributeClusterDimension;
-  cluster.val.clusterDim = {static_cast<unsigned>(a.split), 1, 1};
-  config.attrs = &cluster;
-  config.numAttrs = 1;
+  // The kernel may start while the one ahead of it in the stream ends; it waits before it reads (grid_wait).
+  cudaLaunchAttribute attributes[2]{};
+  attributes[0].id = cudaLaunchAttributeClusterDimension;
+  attributes[0].val.clusterDim = {static_cast<unsigned>(a.split), 1, 1};
+  attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[1].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attributes;
+  config.numAttrs = 2;
   return cudaLaunchKernelEx(&config, product_kernel<O, kColumns>, lane_map, column_map, a);
 }
 
 }  // namespace
 
 cudaError_t launch_nvfp4_product(const Nvfp4& a, const Nvfp4& b, const float* bias, const Dense& out,
-                                 int* status, cudaStream_t stream) {
+                                 bool b_ready, int* status, cudaStream_t stream) {
   return with_type(out.type, [&](auto zero) {
     using O = decltype(zero);
     const Side rows{a.block_scales, a.scale, nullptr, out.stride, static_cast<int32_t>(a.rows), a.per_row};
@@ -413,6 +436,7 @@ cudaError_t launch_nvfp4_product(const Nvfp4& a, const Nvfp4& b, const float* bi
     const bool narrow = b.rows <= 128 && b.rows < a.rows;
     args.lane = narrow ? rows : cols;
     args.column = narrow ? cols : rows;
+    args.lane_ready = b_ready && !narrow;
     const Nvfp4 &x = narrow ? a : b, &y = narrow ? b : a;
     DeviceInfo info;
     const cudaError_t err = device_info(&info);

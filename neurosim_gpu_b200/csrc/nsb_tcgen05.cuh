@@ -18,6 +18,9 @@ __device__ __forceinline__ bool elect_one() {
   return elected != 0;
 }
 
+// Until the kernels ahead in the stream are complete (a launch that may overlap them).
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---------------------------------------------------------------------------
 // mbarriers
 // ---------------------------------------------------------------------------

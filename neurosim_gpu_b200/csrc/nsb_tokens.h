@@ -10,6 +10,20 @@ namespace nsb {
 int set_error(int code, const char* message) noexcept;
 int set_cuda_error(cudaError_t err, const char* where) noexcept;
 
+// Raises a kernel's limit of dynamic shared memory once per device.
+struct SharedLimit {
+  bool raised[64] = {};
+  template <typename K>
+  cudaError_t raise(K* kernel, int bytes) {
+    int device = 0;
+    cudaError_t err = cudaGetDevice(&device);
+    if (err != cudaSuccess || raised[device & 63]) return err;
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    raised[device & 63] = err == cudaSuccess;
+    return err;
+  }
+};
+
 // stimulus.cu
 cudaError_t launch_stimulus_drive(const void* tokens, int token_bytes, int64_t n, const Dense& table,
                                   float scale, const Dense& out, cudaStream_t stream);
@@ -35,8 +49,9 @@ size_t column_sums_workspace_bytes(int64_t rows, int64_t cols);
 cudaError_t launch_column_sums(const Dense& value, float* out, void* workspace, cudaStream_t stream);
 
 // microscale_product.cu
+// b_ready: b was complete before the kernel ahead in the stream started.
 cudaError_t launch_nvfp4_product(const Nvfp4& a, const Nvfp4& b, const float* bias, const Dense& out,
-                                 int* status, cudaStream_t stream);
+                                 bool b_ready, int* status, cudaStream_t stream);
 
 // logits.cu
 struct LogitsArgs {

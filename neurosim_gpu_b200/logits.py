@@ -10,7 +10,7 @@ import ctypes
 
 import torch
 
-from .native import _Logits, _RowValues, dense_matrix, load_library, token_call
+from .native import _Logits, _Matrix, _RowValues, dense_matrix, load_library, token_call
 
 
 def _row_values(value: float | torch.Tensor, name: str, rows: int, device: torch.device) -> _RowValues:
@@ -21,9 +21,7 @@ def _row_values(value: float | torch.Tensor, name: str, rows: int, device: torch
     return _RowValues(value.data_ptr(), value.stride(0) if value.dim() == 1 and value.shape[0] > 1 else 0, 1.0)
 
 
-def _lengths(value: torch.Tensor | None, name: str, rows: int, device: torch.device) -> int | None:
-    if value is None:
-        return None
+def _lengths(value: torch.Tensor, name: str, rows: int, device: torch.device) -> int:
     if (value.dtype != torch.int32 or value.device != device or tuple(value.shape) != (rows,)
             or not value.is_contiguous()):
         raise ValueError(f"{name} must be a contiguous int32 vector with one value per row")
@@ -65,16 +63,17 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
     set where token v is allowed.  ``out`` may be ``logits``.  The choice is the lowest index of a
     row's largest adjusted logit, -1 where nothing is above -inf; a NaN is never chosen.
     """
-    rows, vocabulary = logits.shape if logits.dim() == 2 else (0, 0)
     view = dense_matrix(logits, "logits")
+    rows, vocabulary = view.rows, view.cols
     device = logits.device
-    args = _Logits()
-    args.logits = view
+    args = _Logits(view)
     if out is None:
-        out = torch.empty((rows, vocabulary), device=device, dtype=logits.dtype)
+        out = logits.new_empty((rows, vocabulary))
+        args.out = _Matrix(out.data_ptr(), rows, vocabulary, vocabulary, view.type)
     elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != device:
         raise ValueError("out must have the logits' shape, dtype and device")
-    args.out = view if out is logits else dense_matrix(out, "out")
+    else:
+        args.out = view if out is logits else dense_matrix(out, "out")
     if history is not None:
         if (history.dtype != torch.int32 or history.device != device or history.dim() != 2
                 or history.shape[0] != rows or (history.shape[1] > 1 and history.stride(1) != 1)):
@@ -83,8 +82,10 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
         args.history_length, args.history_stride = history.shape[1], history.stride(0)
     elif lengths is not None or prompt_lengths is not None:
         raise ValueError("lengths need a history")
-    args.lengths = _lengths(lengths, "lengths", rows, device)
-    args.prompt_lengths = _lengths(prompt_lengths, "prompt_lengths", rows, device)
+    if lengths is not None:
+        args.lengths = _lengths(lengths, "lengths", rows, device)
+    if prompt_lengths is not None:
+        args.prompt_lengths = _lengths(prompt_lengths, "prompt_lengths", rows, device)
     args.repetition = _row_values(repetition, "repetition", rows, device)
     args.presence = _row_values(presence, "presence", rows, device)
     args.frequency = _row_values(frequency, "frequency", rows, device)
@@ -92,8 +93,8 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
         args.bias, args.bias_stride = _broadcast(bias, "bias", torch.float32, rows, vocabulary, device)
     if mask is not None:
         args.mask, args.mask_stride = _broadcast(mask, "mask", torch.int32, rows, (vocabulary + 31) // 32, device)
-    choice = torch.empty(rows, device=device, dtype=torch.int64) if choose else None
+    choice = logits.new_empty(rows, dtype=torch.int64) if choose else None
     if choose:
         args.choice = choice.data_ptr()
-    token_call(device, load_library().nsb_adjust_logits, ctypes.byref(args))
+    token_call(logits, load_library().nsb_adjust_logits, ctypes.byref(args))
     return (out, choice) if choose else out

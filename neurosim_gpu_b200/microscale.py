@@ -17,14 +17,12 @@ from __future__ import annotations
 
 import ctypes
 import functools
-from dataclasses import dataclass
 
 import torch
 
-from .native import VALUE_TYPES, _Nvfp4, dense_matrix, load_library, token_call
+from .native import VALUE_TYPES, _Matrix, _Nvfp4, dense_matrix, load_library, token_call
 
 
-@dataclass(frozen=True)
 class Nvfp4Matrix:
     """A packed [rows, columns] matrix; R = rows, K = columns.
 
@@ -32,30 +30,33 @@ class Nvfp4Matrix:
     nibble.  ``block_scales``: uint8 E4M3 [ceil(R / 128), 4 * ceil(K / 256), 512]; tile (i, j) holds
     rows 128 i ... and blocks of 16 columns 4 j ..., the scale of row r and block b at byte
     16 (r % 32) + 4 (r % 128 // 32) + b % 4.  ``scale``: float32 [R] or [1].  Codes and block scales
-    beyond K are zero.
+    beyond K are zero.  The tensors are used as they are, not copied.
     """
 
-    codes: torch.Tensor
-    block_scales: torch.Tensor
-    scale: torch.Tensor
-    columns: int
+    __slots__ = ("codes", "block_scales", "scale", "columns", "_view")
 
-    def __post_init__(self) -> None:
-        codes, scales, scale, columns = self.codes, self.block_scales, self.scale, self.columns
+    def __init__(self, codes: torch.Tensor, block_scales: torch.Tensor, scale: torch.Tensor,
+                 columns: int) -> None:
         if columns < 1:
             raise ValueError("an NVFP4 matrix needs at least one column")
-        rows = codes.shape[0]
-        if codes.dtype != torch.uint8 or tuple(codes.shape) != (rows, (columns + 31) // 32 * 16):
+        shape = codes.shape
+        rows = shape[0] if shape else 0
+        if codes.dtype is not torch.uint8 or shape != (rows, (columns + 31) // 32 * 16):
             raise ValueError("codes must be uint8 [rows, 16 * ceil(columns / 32)]")
-        if (scales.dtype != torch.uint8
-                or tuple(scales.shape) != ((rows + 127) // 128, (columns + 255) // 256 * 4, 512)):
+        if (block_scales.dtype is not torch.uint8
+                or block_scales.shape != ((rows + 127) // 128, (columns + 255) // 256 * 4, 512)):
             raise ValueError("block_scales must be uint8 [ceil(rows / 128), 4 * ceil(columns / 256), 512]")
-        if scale.dtype != torch.float32 or scale.dim() != 1 or scale.shape[0] not in (1, rows):
+        count = scale.numel()
+        if scale.dtype is not torch.float32 or scale.dim() != 1 or (count != 1 and count != rows):
             raise ValueError("scale must be float32 [rows] or [1]")
-        if not (codes.is_cuda and codes.device == scales.device == scale.device):
+        device = codes.get_device()
+        if device < 0 or block_scales.get_device() != device or scale.get_device() != device:
             raise ValueError("codes, block_scales and scale must be on one CUDA device")
-        if not (codes.is_contiguous() and scales.is_contiguous() and scale.is_contiguous()):
+        if not (codes.is_contiguous() and block_scales.is_contiguous() and scale.is_contiguous()):
             raise ValueError("codes, block_scales and scale must be contiguous")
+        self.codes, self.block_scales, self.scale, self.columns = codes, block_scales, scale, columns
+        self._view = _Nvfp4(rows, columns, codes.data_ptr(), shape[1], block_scales.data_ptr(),
+                            scale.data_ptr(), count)
 
     @property
     def rows(self) -> int:
@@ -69,17 +70,14 @@ class Nvfp4Matrix:
     def device(self) -> torch.device:
         return self.codes.device
 
-    def _view(self) -> _Nvfp4:
-        return _Nvfp4(self.codes.shape[0], self.columns, self.codes.data_ptr(), self.codes.shape[1],
-                      self.block_scales.data_ptr(), self.scale.data_ptr(), self.scale.shape[0])
-
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The values the codes stand for: level * (block scale * scale), rounded to ``dtype``."""
         if dtype not in VALUE_TYPES:
             raise ValueError("dtype must be float32, float16 or bfloat16")
-        out = torch.empty(self.shape, device=self.device, dtype=dtype)
-        view, result = self._view(), dense_matrix(out, "out")
-        token_call(self.device, load_library().nsb_nvfp4_dequantize, ctypes.byref(view),
+        rows, columns = self.shape
+        out = self.scale.new_empty((rows, columns), dtype=dtype)
+        result = _Matrix(out.data_ptr(), rows, columns, columns, VALUE_TYPES[dtype])
+        token_call(out, load_library().nsb_nvfp4_dequantize, ctypes.byref(self._view),
                    ctypes.byref(result))
         return out
 
@@ -103,37 +101,39 @@ def _quantize(value: torch.Tensor, per_row: bool, transpose: bool, amax: torch.T
     rows, columns = (view.cols, view.rows) if transpose else (view.rows, view.cols)
     if view.cols < 1 or columns < 1:
         raise ValueError("an NVFP4 matrix needs at least one column")
-    device = value.device
-    codes = torch.empty((rows, (columns + 31) // 32 * 16), device=device, dtype=torch.uint8)
-    scales = torch.empty(((rows + 127) // 128, (columns + 255) // 256 * 4, 512), device=device,
-                         dtype=torch.uint8)
+    codes = value.new_empty((rows, (columns + 31) // 32 * 16), dtype=torch.uint8)
+    scales = value.new_empty(((rows + 127) // 128, (columns + 255) // 256 * 4, 512), dtype=torch.uint8)
+    count = rows if per_row else 1
     # A tensor without rows has the scale of zeros.
-    scale = (torch.empty if rows else torch.ones)(rows if per_row else 1, device=device,
-                                                  dtype=torch.float32)
+    scale = value.new_empty(count, dtype=torch.float32) if rows else value.new_ones(count, dtype=torch.float32)
     packed = Nvfp4Matrix(codes, scales, scale, columns)
     lib = load_library()
-    result = packed._view()
-    size = lib.nsb_nvfp4_quantize_workspace_size(view.rows, view.cols, int(transpose), scale.shape[0])
-    workspace = torch.empty(size, device=device, dtype=torch.uint8) if size else None
-    token_call(device, lib.nsb_nvfp4_quantize, ctypes.byref(view), int(transpose),
-               ctypes.byref(result), None if amax is None else amax.data_ptr(), int(given),
+    # A row's own scale needs no workspace; see nsb_nvfp4_quantize_workspace_size.
+    size = 0 if per_row and not transpose else lib.nsb_nvfp4_quantize_workspace_size(
+        view.rows, view.cols, int(transpose), count)
+    workspace = value.new_empty(size, dtype=torch.uint8) if size else None
+    token_call(value, lib.nsb_nvfp4_quantize, ctypes.byref(view), transpose,
+               ctypes.byref(packed._view), None if amax is None else amax.data_ptr(), given,
                workspace.data_ptr() if size else None, size)
     return packed
 
 
 @functools.lru_cache(maxsize=None)
-def _status(device: torch.device) -> torch.Tensor:
-    """The word that products on ``device`` write an error code to (never inside a capture)."""
+def _status(device: int) -> torch.Tensor:
+    """The word that products on a device write an error code to (never inside a capture)."""
     with torch.inference_mode(False):
-        return torch.zeros(1, device=device, dtype=torch.int32)
+        return torch.zeros(1, device=torch.device("cuda", device), dtype=torch.int32)
+
+
+@functools.lru_cache(maxsize=None)
+def _status_pointer(device: int) -> int:
+    return _status(device).data_ptr()
 
 
 def check_product_status(device: torch.device | str = "cuda") -> None:
     """Raise if a product on ``device`` gave up on a bounded wait (reads the device)."""
-    device = torch.device(device)
-    if device.index is None:
-        device = torch.device("cuda", torch.cuda.current_device())
-    code = int(_status(device).item())
+    index = torch.device(device).index
+    code = int(_status(torch.cuda.current_device() if index is None else index).item())
     if code:
         raise RuntimeError(f"NVFP4 product pipeline timeout (code {code})")
 
@@ -146,33 +146,56 @@ def nvfp4_product(a: Nvfp4Matrix, b: Nvfp4Matrix, *, bias: torch.Tensor | None =
     ``bias``: float32 [N].  The result is rounded once to ``dtype`` and depends on the operands
     alone (the same call gives the same bits).  ``out`` receives it where given (contiguous rows).
     """
-    if a.columns != b.columns or a.device != b.device:
+    m, n, device = a.rows, b.rows, a.scale.get_device()
+    if a.columns != b.columns or device != b.scale.get_device():
         raise ValueError("the operands must have the same number of columns and the same device")
-    if b.rows < 1:
+    if n < 1:
         raise ValueError("the second operand needs at least one row")
-    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (b.rows,)
-                             or bias.device != a.device or not bias.is_contiguous()):
-        raise ValueError("bias must be a contiguous float32 [N] on the operands' device")
+    _check_bias(bias, n, device)
     if out is None:
         if dtype not in VALUE_TYPES:
             raise ValueError("dtype must be float32, float16 or bfloat16")
-        out = torch.empty((a.rows, b.rows), device=a.device, dtype=dtype)
-    elif tuple(out.shape) != (a.rows, b.rows) or out.dtype != dtype or out.device != a.device:
+        out = a.scale.new_empty((m, n), dtype=dtype)
+    elif out.shape != (m, n) or out.dtype != dtype or out.get_device() != device:
         raise ValueError("out must be [M, N] of the given dtype on the operands' device")
-    x, y, result = a._view(), b._view(), dense_matrix(out, "out")
-    token_call(a.device, load_library().nsb_nvfp4_product, ctypes.byref(x), ctypes.byref(y),
-               None if bias is None else bias.data_ptr(), ctypes.byref(result),
-               _status(a.device).data_ptr())
+    result = dense_matrix(out, "out")
+    token_call(out, load_library().nsb_nvfp4_product, ctypes.byref(a._view), ctypes.byref(b._view),
+               None if bias is None else bias.data_ptr(), ctypes.byref(result), _status_pointer(device))
+    return out
+
+
+def _check_bias(bias: torch.Tensor | None, n: int, device: int) -> None:
+    if bias is not None and (bias.dtype is not torch.float32 or bias.shape != (n,)
+                             or bias.get_device() != device or not bias.is_contiguous()):
+        raise ValueError("bias must be a contiguous float32 [N] on the operands' device")
+
+
+def _readout(state: torch.Tensor, weight: Nvfp4Matrix, bias: torch.Tensor | None,
+             dtype: torch.dtype) -> torch.Tensor:
+    """[M, K] states through packed weights in one call of the library."""
+    view = dense_matrix(state, "state")
+    rows, columns, n, device = view.rows, view.cols, weight.rows, state.get_device()
+    if weight.scale.get_device() != device or n < 1:
+        raise ValueError("weights must have at least one row and be on the states' device")
+    _check_bias(bias, n, device)
+    out = state.new_empty((rows, n), dtype=dtype)
+    result = _Matrix(out.data_ptr(), rows, n, n, VALUE_TYPES[dtype])
+    # Codes, block scales and scale of the states: nsb_nvfp4_readout_workspace_size.
+    size = rows * ((columns + 31) // 32 * 16) + (rows + 127) // 128 * ((columns + 255) // 256) * 2048 + 4 * rows
+    workspace = state.new_empty(size, dtype=torch.uint8)
+    token_call(state, load_library().nsb_nvfp4_readout, ctypes.byref(view), ctypes.byref(weight._view),
+               None if bias is None else bias.data_ptr(), ctypes.byref(result), workspace.data_ptr(), size,
+               _status_pointer(device))
     return out
 
 
 def _column_sums(value: torch.Tensor) -> torch.Tensor:
     view = dense_matrix(value, "value")
-    out = torch.empty(value.shape[1], device=value.device, dtype=torch.float32)
+    out = value.new_empty(view.cols, dtype=torch.float32)
     lib = load_library()
-    size = lib.nsb_column_sums_workspace_size(*value.shape)
-    workspace = torch.empty(size, device=value.device, dtype=torch.uint8)
-    token_call(value.device, lib.nsb_column_sums, ctypes.byref(view), out.data_ptr(),
+    size = lib.nsb_column_sums_workspace_size(view.rows, view.cols)
+    workspace = value.new_empty(size, dtype=torch.uint8)
+    token_call(value, lib.nsb_column_sums, ctypes.byref(view), out.data_ptr(),
                workspace.data_ptr(), size)
     return out
 
@@ -227,21 +250,22 @@ def nvfp4_readout(state: torch.Tensor, weight: Nvfp4Matrix | torch.Tensor,
     dtype = state.dtype if dtype is None else dtype
     if dtype not in VALUE_TYPES:
         raise ValueError("dtype must be float32, float16 or bfloat16")
-    if state.dim() < 1 or state.shape[-1] != (weight.columns if isinstance(weight, Nvfp4Matrix)
-                                              else weight.shape[-1]):
+    packed = isinstance(weight, Nvfp4Matrix)
+    shape = state.shape
+    if not shape or shape[-1] != (weight.columns if packed else weight.shape[-1]):
         raise ValueError("states must be [..., K] for weights [N_out, K]")
-    flat = state if state.dim() == 2 else state.reshape(-1, state.shape[-1])
-    if flat.shape[0] > 1 and flat.stride(0) < flat.shape[1] or flat.shape[1] > 1 and flat.stride(1) != 1:
+    flat = state if len(shape) == 2 else state.reshape(-1, shape[-1])
+    row_stride, stride = flat.stride()
+    if (stride != 1 and shape[-1] > 1) or (row_stride < shape[-1] and flat.shape[0] > 1):
         flat = flat.contiguous()  # e.g. the neuron-major states of a batch
     wants = torch.is_grad_enabled() and (state.requires_grad
                                          or (bias is not None and bias.requires_grad))
-    if isinstance(weight, Nvfp4Matrix):
+    if packed:
         if wants:
             raise ValueError("packed weights take no gradients: pass floating-point weights")
-        result = nvfp4_product(quantize_nvfp4(flat), weight, bias=bias, dtype=dtype)
+        result = _readout(flat, weight, bias, dtype)
     elif wants or (torch.is_grad_enabled() and weight.requires_grad):
         result = _Readout.apply(flat, weight, bias, dtype)
     else:
-        result = nvfp4_product(quantize_nvfp4(flat), quantize_nvfp4(weight, per="tensor"), bias=bias,
-                               dtype=dtype)
-    return result if state.dim() == 2 else result.view(*state.shape[:-1], result.shape[1])
+        result = _readout(flat, _quantize(weight, False, False), bias, dtype)
+    return result if len(shape) == 2 else result.view(*shape[:-1], result.shape[1])

@@ -169,7 +169,8 @@ EXPORTED_SYMBOLS = ("nsb_dendritic_step", "nsb_csr_propagate",
                     "nsb_tiled_propagate_rows_gated", "nsb_stimulus_drive",
                     "nsb_stimulus_gradient_workspace_size", "nsb_stimulus_gradient",
                     "nsb_nvfp4_quantize_workspace_size", "nsb_nvfp4_quantize",
-                    "nsb_nvfp4_dequantize", "nsb_nvfp4_product", "nsb_column_sums_workspace_size",
+                    "nsb_nvfp4_dequantize", "nsb_nvfp4_product", "nsb_nvfp4_readout_workspace_size",
+                    "nsb_nvfp4_readout", "nsb_column_sums_workspace_size",
                     "nsb_column_sums", "nsb_adjust_logits", "nsb_last_error", "nsb_abi_version")
 
 
@@ -268,6 +269,9 @@ def load_library() -> ctypes.CDLL:
     lib.nsb_nvfp4_quantize.argtypes = [p(_Matrix), i32, p(_Nvfp4), ptr, i32, ptr, size, ptr]
     lib.nsb_nvfp4_dequantize.argtypes = [p(_Nvfp4), p(_Matrix), ptr]
     lib.nsb_nvfp4_product.argtypes = [p(_Nvfp4), p(_Nvfp4), ptr, p(_Matrix), ptr, ptr]
+    lib.nsb_nvfp4_readout_workspace_size.argtypes = [i64, i64]
+    lib.nsb_nvfp4_readout_workspace_size.restype = size
+    lib.nsb_nvfp4_readout.argtypes = [p(_Matrix), p(_Nvfp4), ptr, p(_Matrix), ptr, size, ptr, ptr]
     lib.nsb_column_sums_workspace_size.argtypes = [i64, i64]
     lib.nsb_column_sums_workspace_size.restype = size
     lib.nsb_column_sums.argtypes = [p(_Matrix), ptr, ptr, size, ptr]
@@ -322,22 +326,30 @@ def dense_matrix(value: torch.Tensor, name: str) -> _Matrix:
     kind = VALUE_TYPES.get(value.dtype)
     if kind is None or not value.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor of float32, float16 or bfloat16")
-    if value.dim() != 2:
+    shape = value.shape
+    if len(shape) != 2:
         raise ValueError(f"{name} must have two dimensions")
-    rows, cols = value.shape
+    rows, cols = shape
     row_stride, stride = value.stride()
-    if rows > 0 and ((cols > 1 and stride != 1) or (rows > 1 and row_stride < cols)):
+    if rows > 0 and ((stride != 1 and cols > 1) or (row_stride < cols and rows > 1)):
         raise ValueError(f"{name} must have contiguous rows that do not overlap")
-    return _Matrix(value.data_ptr(), rows, cols, max(row_stride, cols), kind)
+    return _Matrix(value.data_ptr(), rows, cols, row_stride if row_stride > cols else cols, kind)
 
 
-def token_call(device: torch.device, function, *arguments) -> None:
-    """Call a token operator of the library on the current stream of ``device``."""
-    if device.index == torch.cuda.current_device():
-        status = function(*arguments, torch.cuda.current_stream(device).cuda_stream)
+# The current stream as a pointer and the current device: what torch.cuda.current_stream() and
+# current_device() return, without building a Stream object for every call.
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+
+
+def token_call(tensor: torch.Tensor, function, *arguments) -> None:
+    """Call a token operator of the library on the current stream of the tensor's device."""
+    device = tensor.get_device()
+    if device == _current_device():
+        status = function(*arguments, _raw_stream(device) if _raw_stream is not None else _stream(tensor.device))
     else:
         with torch.cuda.device(device):
-            status = function(*arguments, torch.cuda.current_stream(device).cuda_stream)
+            status = function(*arguments, _stream(tensor.device))
     if status != 0:
         _raise_on_status(load_library(), status)
 

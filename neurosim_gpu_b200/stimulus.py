@@ -14,13 +14,13 @@ import ctypes
 
 import torch
 
-from .native import VALUE_TYPES, dense_matrix, load_library, token_call
+from .native import VALUE_TYPES, _Matrix, dense_matrix, load_library, token_call
 
 
-def _tokens(tokens: torch.Tensor, device: torch.device) -> torch.Tensor:
-    if tokens.dtype not in (torch.int32, torch.int64):
+def _tokens(tokens: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
+    if tokens.dtype is not torch.int64 and tokens.dtype is not torch.int32:
         raise ValueError("tokens must be int32 or int64")
-    if tokens.device != device:
+    if tokens.get_device() != like.get_device():
         raise ValueError("tokens must be on the table's CUDA device")
     return tokens if tokens.is_contiguous() else tokens.contiguous()
 
@@ -28,17 +28,17 @@ def _tokens(tokens: torch.Tensor, device: torch.device) -> torch.Tensor:
 def _drive(tokens: torch.Tensor, table: torch.Tensor, scale: float, dtype: torch.dtype,
            out: torch.Tensor | None) -> torch.Tensor:
     view = dense_matrix(table, "table")
-    tokens = _tokens(tokens, table.device)
-    shape = (*tokens.shape, table.shape[1])
+    tokens = _tokens(tokens, table)
+    shape = (*tokens.shape, view.cols)
     if out is None:
-        out = torch.empty(shape, device=table.device, dtype=dtype)
+        out = table.new_empty(shape, dtype=dtype)
     elif out.shape != shape or out.dtype != dtype or out.device != table.device:
         raise ValueError("out must be a tensor of the drive's shape, dtype and device")
     elif not out.is_contiguous():
         raise ValueError("out must be contiguous")
-    rows = dense_matrix(out.view(tokens.numel(), table.shape[1]), "out")
-    token_call(table.device, load_library().nsb_stimulus_drive, tokens.data_ptr(),
-               tokens.element_size(), ctypes.byref(view), float(scale), ctypes.byref(rows))
+    rows = _Matrix(out.data_ptr(), tokens.numel(), view.cols, view.cols, VALUE_TYPES[dtype])
+    token_call(table, load_library().nsb_stimulus_drive, tokens.data_ptr(),
+               tokens.element_size(), ctypes.byref(view), scale, ctypes.byref(rows))
     return out
 
 
@@ -73,7 +73,7 @@ def stimulus_drive(tokens: torch.Tensor, table: torch.Tensor, *, scale: float = 
     if table.requires_grad and torch.is_grad_enabled():
         if out is not None:
             raise ValueError("out cannot be given where the table requires a gradient")
-        return _StimulusDrive.apply(tokens, table, float(scale), dtype)
+        return _StimulusDrive.apply(tokens, table, scale, dtype)
     return _drive(tokens, table, scale, dtype, out)
 
 
@@ -94,16 +94,16 @@ def stimulus_gradient(tokens: torch.Tensor, grad: torch.Tensor, rows: int, *, sc
         raise ValueError("grad must be [*tokens.shape, N]")
     if rows < 0:
         raise ValueError("rows must not be negative")
-    tokens = _tokens(tokens, grad.device)
+    tokens = _tokens(tokens, grad)
     flat = grad.reshape(tokens.numel(), grad.shape[-1])
     if flat.shape[1] > 1 and flat.stride(1) != 1 or flat.shape[0] > 1 and flat.stride(0) < flat.shape[1]:
         flat = flat.contiguous()  # e.g. the expanded gradient of a sum
     view = dense_matrix(flat, "grad")
-    out = torch.empty((rows, flat.shape[1]), device=grad.device, dtype=dtype)
-    result = dense_matrix(out, "out")
+    out = grad.new_empty((rows, view.cols), dtype=dtype)
+    result = _Matrix(out.data_ptr(), rows, view.cols, view.cols, VALUE_TYPES[dtype])
     lib = load_library()
-    size = lib.nsb_stimulus_gradient_workspace_size(*flat.shape)
-    workspace = torch.empty(size, device=grad.device, dtype=torch.uint8)
-    token_call(grad.device, lib.nsb_stimulus_gradient, tokens.data_ptr(), tokens.element_size(),
-               ctypes.byref(view), float(scale), ctypes.byref(result), workspace.data_ptr(), size)
+    size = lib.nsb_stimulus_gradient_workspace_size(view.rows, view.cols)
+    workspace = grad.new_empty(size, dtype=torch.uint8)
+    token_call(grad, lib.nsb_stimulus_gradient, tokens.data_ptr(), tokens.element_size(),
+               ctypes.byref(view), scale, ctypes.byref(result), workspace.data_ptr(), size)
     return out

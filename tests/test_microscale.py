@@ -113,6 +113,16 @@ def test_entry_points_refuse_bad_arguments():
         assert product(**bad) == -1, bad
     assert product(a=packed(rows=0, codes=None, scales=None, scale=None),
                    out=native._Matrix(None, 0, 6, 6, 0)) == 0
+    state, size = native._Matrix(p, 4, 40, 40, 0), lib.nsb_nvfp4_readout_workspace_size(4, 40)
+    assert size == 4 * 32 + 2048 + 16
+
+    def readout(state=state, weight=packed(rows=6), out=out, workspace=p, size=size, bias=None):
+        return lib.nsb_nvfp4_readout(ctypes.byref(state), ctypes.byref(weight), bias, ctypes.byref(out), workspace, size,
+                                     None, None)
+
+    for bad in ({"weight": packed(rows=7)}, {"weight": packed(rows=6, cols=41)}, {"bias": p + 2}, {"state": native._Matrix(p, 5, 40, 40, 0)}):
+        assert readout(**bad) == -1, bad
+    assert readout(size=size - 1) == -3 and readout(workspace=None) == -3 and readout(workspace=p + 8) == -3
     assert lib.nsb_nvfp4_dequantize(ctypes.byref(packed()), ctypes.byref(native._Matrix(p, 4, 41, 41, 0)), None) == -1
     assert lib.nsb_column_sums(ctypes.byref(value), None, p, 10**6, None) == -1
     assert lib.nsb_column_sums(ctypes.byref(value), p, p, 1, None) == -3
