@@ -14,12 +14,14 @@ from .precision import PRECISIONS, encode_sparse_weights, quantize_dequantize
 from .runtime import (NativeDendriticMatrixRuntime, NativeDendriticPELSRuntime, RuntimeStats,
                       validate_emission_threshold)
 from .stimulus import stimulus_drive, stimulus_gradient
+from .tokens import generate_tokens
 from .topology import SparseTopology, random_topology
 
 __all__ = [
     "DendriticDynamics", "Dynamics", "NativeDendriticMatrixRuntime",
     "NativeDendriticPELSRuntime", "Nvfp4Matrix", "PRECISIONS", "RuntimeStats", "SparseTopology",
-    "adjust_logits", "check_product_status", "encode_sparse_weights", "load_native_extension",
+    "adjust_logits", "check_product_status", "encode_sparse_weights", "generate_tokens",
+    "load_native_extension",
     "nvfp4_product", "nvfp4_readout", "quantize_dequantize", "quantize_nvfp4",
     "random_topology", "stimulus_drive", "stimulus_gradient", "validate_emission_threshold",
 ]

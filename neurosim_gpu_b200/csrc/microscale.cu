@@ -65,14 +65,24 @@ struct Words {
   }
 };
 
-// The values from column c of a row, zeros beyond `cols`.  kVec: rows start on 16 bytes.  Else a row
+// The values from column c of a row, zeros beyond `cols`.  kVec: rows start on that many bytes, 32 or 16
+// (a lane's 64 bytes of float32 in two loads instead of four halve the work of L1).  Where it is 0 a row
 // starts `lead` values after a multiple of 16 bytes: the words are cut out of the aligned vectors
 // around them, as long as these lie within the matrix, [first, last).
-template <typename T, bool kVec>
+template <typename T, int kVec>
 __device__ __forceinline__ Words<T> load_block(const T* row, int64_t c, int64_t cols, int lead, const T* first, const T* last) {
   constexpr int P = 16 / static_cast<int>(sizeof(T)), kVectors = 16 / P;
   Words<T> r;
-  if (kVec && c + 16 <= cols) {
+  if (kVec == 32 && c + 16 <= cols) {
+#pragma unroll
+    for (int q = 0; q < kVectors / 2; ++q)
+      asm("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+          : "=r"(r.w[8 * q]), "=r"(r.w[8 * q + 1]), "=r"(r.w[8 * q + 2]), "=r"(r.w[8 * q + 3]), "=r"(r.w[8 * q + 4]),
+            "=r"(r.w[8 * q + 5]), "=r"(r.w[8 * q + 6]), "=r"(r.w[8 * q + 7])
+          : "l"(row + c + 2 * q * P));
+    return r;
+  }
+  if (kVec == 16 && c + 16 <= cols) {
 #pragma unroll
     for (int q = 0; q < kVectors; ++q) {
       const uint4 x = __ldg(reinterpret_cast<const uint4*>(row + c) + q);
@@ -142,7 +152,7 @@ __device__ __forceinline__ void write_block(const Nvfp4& out, int64_t r, int64_t
 // 2^per_row threads (16 ... 256) take a row, the CTA's 256 several rows; or a cluster of 2^cluster CTAs
 // takes one.  B blocks per thread stay in registers, further ones are read twice.  `given`: the matrix's amax (its bits), or null
 // for each row's own; `most`: receives the matrix's amax (zero before), or null.
-template <typename T, bool kVec, int B>
+template <typename T, int kVec, int B>
 __global__ void __launch_bounds__(kRowThreads)
 quantize_rows_kernel(Dense x, Nvfp4 out, const unsigned int* given, unsigned int* most, int per_row, int cluster, unsigned work) {
   __shared__ unsigned int best_of[kRowThreads / 32];
@@ -221,8 +231,9 @@ quantize_columns_kernel(Dense x, Nvfp4 out, const unsigned int* amax) {
   auto place = [&](int at) -> Pack<T, P>& { return *reinterpret_cast<Pack<T, P>*>(tile + at / kAcross * kRowBytes + at % kAcross * sizeof(Pack<T, P>)); };
   __shared__ unsigned long long codes[kTileCols][kTileRows / 16 + 1];
   __shared__ uint8_t scales[kTileCols][kTileRows / 16 + 4];
-  const int64_t across = (x.cols + 127) / 128 * 2;  // the result's rows are padded to 128 for their scales
-  const int64_t c0 = blockIdx.x % across * kTileCols, r0 = blockIdx.x / across * kTileRows;
+  const unsigned across = static_cast<unsigned>((x.cols + 127) / 128 * 2);  // the result's rows are padded to 128 for their scales
+  const unsigned down = blockIdx.x / across;
+  const int64_t c0 = static_cast<int64_t>(blockIdx.x - down * across) * kTileCols, r0 = static_cast<int64_t>(down) * kTileRows;
   const T* data = static_cast<const T*>(x.data);
   Pack<T, P> v[kVec ? kLoads : 1];
 #pragma unroll
@@ -431,17 +442,41 @@ dequantize_kernel(Nvfp4 in, Dense out, unsigned chunks) {
   }
 }
 
-// Sums of the columns over rows [blockIdx.y * span, + span), in ascending rows, to row blockIdx.y of `sums`.
-template <typename T>
+// Sums of the columns over rows [blockIdx.y * span, + span) to row blockIdx.y of `sums`.  A CTA takes 32 * P
+// columns; its 8 warps take every 8th row, and are added in order.
+template <typename T, bool kVec>
 __global__ void __launch_bounds__(kAmaxThreads)
 column_sums_kernel(Dense x, int64_t span, float* sums) {
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * kAmaxThreads + threadIdx.x;
-  if (c >= x.cols) return;
+  constexpr int P = kVec ? 16 / static_cast<int>(sizeof(T)) : 1;
+  constexpr int kWarps = kAmaxThreads / 32;
+  __shared__ float all[kWarps][32 * P];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t c = (static_cast<int64_t>(blockIdx.x) * 32 + lane) * P;
   const int64_t last = min(x.rows, (blockIdx.y + 1) * span);
-  float sum = 0.0f;
+  const T* data = static_cast<const T*>(x.data);
+  float sum[P] = {};
+  if (c + P <= x.cols) {
 #pragma unroll 8
-  for (int64_t r = blockIdx.y * span; r < last; ++r) sum += Values<T>::up(static_cast<const T*>(x.data)[r * x.stride + c]);
-  sums[blockIdx.y * x.cols + c] = sum;
+    for (int64_t r = blockIdx.y * span + warp; r < last; r += kWarps) {
+      const Pack<T, P> v = load_pack<T, P>(data + r * x.stride + c);
+#pragma unroll
+      for (int k = 0; k < P; ++k) sum[k] += Values<T>::up(v.v[k]);
+    }
+  } else {
+    for (int64_t r = blockIdx.y * span + warp; r < last; r += kWarps)
+      for (int k = 0; k < P; ++k)
+        if (c + k < x.cols) sum[k] += Values<T>::up(data[r * x.stride + c + k]);
+  }
+#pragma unroll
+  for (int k = 0; k < P; ++k) all[warp][lane * P + k] = sum[k];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * P; i += kAmaxThreads) {
+    const int64_t to = static_cast<int64_t>(blockIdx.x) * 32 * P + i;
+    float total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) total += all[w][i];
+    if (to < x.cols) sums[blockIdx.y * x.cols + to] = total;
+  }
 }
 
 __global__ void __launch_bounds__(kAmaxThreads)
@@ -454,8 +489,8 @@ join_sums_kernel(const float* sums, int64_t parts, int64_t cols, float* out) {
   out[c] = sum;
 }
 
-// Rows per partial sum: short enough to fill the GPU, and at most 1,024 parts.
-int64_t sum_span(int64_t rows) { return std::max<int64_t>(64, (rows + 1023) / 1024); }
+// Rows per partial sum: short enough to fill the GPU, and at most 64 parts.
+int64_t sum_span(int64_t rows) { return std::max<int64_t>(64, (rows + 63) / 64); }
 
 unsigned ceil_div(int64_t a, int64_t b) { return static_cast<unsigned>((a + b - 1) / b); }
 
@@ -478,25 +513,26 @@ cudaError_t amax_pass(Dense x, bool columns, unsigned int* amax, cudaStream_t st
   }
   if (x.stride == x.cols) x = {x.data, 1, x.rows * x.cols, x.rows * x.cols, x.type};
   const unsigned across = ceil_div(std::max<int64_t>(x.cols / P, 1), kAmaxThreads * 4);
-  const unsigned most = static_cast<unsigned>(info.sm_count) * 8;
+  const unsigned most = static_cast<unsigned>(info.sm_count) * 32;
   const dim3 grid(std::min(across, most), static_cast<unsigned>(std::min<int64_t>(x.rows, std::max(1u, most / across))));
   amax_kernel<T, kVec><<<grid, kAmaxThreads, 0, stream>>>(x, amax);
   return cudaGetLastError();
 }
 
-template <typename T, bool kVec>
+template <typename T, int kVec>
 cudaError_t quantize_rows(const Dense& x, const Nvfp4& out, const unsigned int* given, unsigned int* most, cudaStream_t stream) {
   DeviceInfo info;
   cudaError_t err = device_info(&info);
   if (err != cudaSuccess) return err;
   const int64_t blocks = block_scale_tiles(x.cols) * 4;
-  // Two blocks to a thread; a long row is shared by a cluster while there are SMs for it, then held four
-  // blocks to a thread, then shared by up to eight CTAs, then read twice.
-  int per_row = 4, cluster = 0, held = blocks > 16 ? 2 : 1;
-  while (1 << per_row < kRowThreads && blocks > int64_t{held} << per_row) ++per_row;
-  while (cluster < 3 && blocks > int64_t{held} << (per_row + cluster) && x.rows << (cluster + 1) <= info.sm_count) ++cluster;
-  if (blocks > int64_t{held} << (per_row + cluster)) held = 4;
-  while (cluster < 3 && blocks > int64_t{held} << (per_row + cluster)) ++cluster;
+  // Two or three blocks to a thread (up to four are held); a long row is shared by a cluster while there
+  // are SMs for it, then by up to eight CTAs where four blocks do not hold it, then read twice.
+  int per_row = 4, cluster = 0;
+  while (1 << per_row < kRowThreads && blocks > int64_t{3} << per_row) ++per_row;
+  while (cluster < 3 && blocks > int64_t{2} << (per_row + cluster) && x.rows << (cluster + 1) <= info.sm_count) ++cluster;
+  while (cluster < 3 && blocks > int64_t{4} << (per_row + cluster)) ++cluster;
+  if (cluster > 0) per_row = 8;  // a cluster's CTAs are whole
+  const int held = blocks <= int64_t{1} << (per_row + cluster) ? 1 : blocks <= int64_t{2} << (per_row + cluster) ? 2 : 4;
   const int64_t grid = cluster > 0 ? x.rows << cluster : ((x.rows << per_row) + kRowThreads - 1) / kRowThreads;
   const int64_t fill = x.rows % 128 ? ((blocks + 63) / 64 + (1 << cluster) - 1) >> cluster << cluster : 0;
   if (grid + fill > 0x7fffffff) return cudaErrorInvalidConfiguration;
@@ -530,13 +566,15 @@ cudaError_t launch_nvfp4_quantize(const Dense& value, bool transpose, const Nvfp
       const bool by_row = out.per_row && !transpose;
       // The words that the scales come from: one per column of a transpose, or the matrix's.
       unsigned int* words = out.per_row && transpose ? static_cast<unsigned int*>(workspace) : amax ? amax : static_cast<unsigned int*>(workspace);
+      const bool wide = rows_aligned(value, sizeof(T), 32);
+      auto* rows = !kVec ? quantize_rows<T, 0> : wide ? quantize_rows<T, 32> : quantize_rows<T, 16>;
       if (by_row) {
         if (amax && (err = cudaMemsetAsync(amax, 0, 4, stream)) != cudaSuccess) return err;
-        return quantize_rows<T, kVec>(value, out, nullptr, amax, stream);
+        return rows(value, out, nullptr, amax, stream);
       }
       if (out.per_row || !amax_given)
         if ((err = amax_pass<T, kVec>(value, out.per_row, words, stream)) != cudaSuccess) return err;
-      if (!transpose) return quantize_rows<T, kVec>(value, out, words, nullptr, stream);
+      if (!transpose) return rows(value, out, words, nullptr, stream);
       const int64_t grid = (value.cols + 127) / 128 * 2 * (block_scale_tiles(value.rows) / 2);
       if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
       quantize_columns_kernel<T, kVec><<<static_cast<unsigned>(grid), kTileThreads, 0, stream>>>(value, out, words);
@@ -573,13 +611,15 @@ cudaError_t launch_column_sums(const Dense& value, float* out, void* workspace, 
     using T = decltype(zero);
     auto* sums = static_cast<float*>(workspace);
     const int64_t span = sum_span(value.rows), parts = (value.rows + span - 1) / span;
-    const dim3 grid(ceil_div(value.cols, kAmaxThreads), static_cast<unsigned>(parts));
     if (parts > 0) {  // no rows: the sums are zero
-      column_sums_kernel<T><<<grid, kAmaxThreads, 0, stream>>>(value, span, sums);
+      const bool vec = rows_aligned(value, sizeof(T), 16);
+      const dim3 grid(ceil_div(value.cols, vec ? 512 / sizeof(T) : 32), static_cast<unsigned>(parts));
+      auto* kernel = vec ? column_sums_kernel<T, true> : column_sums_kernel<T, false>;
+      kernel<<<grid, kAmaxThreads, 0, stream>>>(value, span, sums);
       const cudaError_t err = cudaGetLastError();
       if (err != cudaSuccess) return err;
     }
-    join_sums_kernel<<<grid.x, kAmaxThreads, 0, stream>>>(sums, parts, value.cols, out);
+    join_sums_kernel<<<ceil_div(value.cols, kAmaxThreads), kAmaxThreads, 0, stream>>>(sums, parts, value.cols, out);
     return cudaGetLastError();
   });
 }
