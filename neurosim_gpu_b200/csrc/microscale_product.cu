@@ -16,6 +16,12 @@
 // for the next tile, and write it.  The scales of a stage have tensor memory of their own, reused
 // only after the stage's products are complete.
 //
+// Large products run on pairs of CTAs (tcgen05 cta_group::2): a tile of 256 lanes x 256 columns, of which
+// each CTA holds 128 lanes' sums and loads its 128 lanes' codes and half of the columns'.  A CTA of its
+// own takes 54 KB from L2 per K tile, at 64 bytes a cycle longer than its products do (860 cycles against
+// 512 of the tensor core); one of a pair takes 38 KB.  The first CTA issues for both, after the second
+// has passed on that its own loads are in.
+//
 // Where there are too few tiles for the GPU, a cluster of 2, 4 or 8 CTAs shares a tile along K: each
 // leaves its float32 partial sums in its shared memory, and each adds a part of the columns of all
 // of them in rank order (deterministic) over distributed shared memory.
@@ -39,11 +45,13 @@ constexpr int kMostShared = 232448;   // dynamic shared memory of a CTA
 constexpr int kLeastShared = 120000;  // more than half an SM's: one CTA per SM, so tensor memory is free
 constexpr int kHeader = 4096;         // barriers, column scales; the stages follow, 1,024-byte aligned
 
-// What a tile of 128 lanes x kColumns columns takes.
-template <int kColumns>
+// What a tile of 128 lanes (of a pair 2 x 128) x kColumns columns takes of a CTA.
+template <int kColumns, bool kPair>
 struct Shape {
   static constexpr int kBlocks = (kColumns + 127) / 128;  // of 128 rows of block scales
-  static constexpr int kStageBytes = kLaneBytes + kColumns * kTileBytes + kScaleBytes * (1 + kBlocks);
+  static constexpr int kColumnRows = kPair ? kColumns / 2 : kColumns;  // of the column operand's codes
+  static constexpr int kColumnBytes = kColumnRows * kTileBytes;
+  static constexpr int kStageBytes = kLaneBytes + kColumnBytes + kScaleBytes * (1 + kBlocks);
   static constexpr int kSlot = 16 * (1 + kBlocks);        // tensor memory columns of a stage's scales
   static constexpr int kSums = kColumns <= 128 ? 2 : 1;   // accumulators
   static constexpr int kStages = std::min({8, (kMostShared - kHeader) / kStageBytes, (kTmemColumns - kSums * kColumns) / kSlot});
@@ -69,13 +77,14 @@ struct ProductArgs {
   void* out;
   int64_t scale_tiles;  // 512-byte tiles per 128 rows
   int32_t k_tiles, split;
-  int32_t lane_tiles, column_tiles;
+  int32_t lane_tiles, column_tiles;  // lane tiles of 128, of pairs 256
   bool lane_ready;  // the operand along the lanes was complete before the kernel ahead of this one started
   int* status;
 };
 
 struct Header {
   uint64_t full[8], empty[8];
+  uint64_t peer_full[8];  // of a pair's first CTA: the second's loads
   uint64_t sum_full[2], sum_empty[2], drained;
   uint32_t tmem;
   int aborted;
@@ -116,39 +125,49 @@ struct Ring {
   }
 };
 
-template <typename O, int kColumns>
-__global__ void __launch_bounds__(Shape<kColumns>::kThreads, 1)
+template <typename O, int kColumns, bool kPair>
+__global__ void __launch_bounds__(Shape<kColumns, kPair>::kThreads, 1)
 product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_constant__ CUtensorMap column_map,
                const __grid_constant__ ProductArgs a) {
-  using S = Shape<kColumns>;
+  using S = Shape<kColumns, kPair>;
   extern __shared__ __align__(1024) uint8_t shared[];
   Header& h = *reinterpret_cast<Header*>(shared);
   uint8_t* stages = shared + kHeader;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   volatile int* aborted = &h.aborted;
   int rank = 0;
-  if (a.split > 1) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  if (kPair || a.split > 1) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   const int tiles = a.lane_tiles * a.column_tiles;
-  const int first = blockIdx.x / a.split, step = gridDim.x / a.split;
-  const int k0 = static_cast<int>(static_cast<int64_t>(a.k_tiles) * rank / a.split);
-  const int k1 = static_cast<int>(static_cast<int64_t>(a.k_tiles) * (rank + 1) / a.split);
+  const int group = kPair ? 2 : a.split;  // CTAs that share a tile: a pair its lanes, others its K tiles
+  const int first = blockIdx.x / group, step = gridDim.x / group;
+  const int k0 = kPair ? 0 : static_cast<int>(static_cast<int64_t>(a.k_tiles) * rank / group);
+  const int k1 = kPair ? a.k_tiles : static_cast<int>(static_cast<int64_t>(a.k_tiles) * (rank + 1) / group);
+  // A pair's second 128 lanes may lie beyond the operand: any scales do for them.
+  auto lane_scale_block = [&](int lane_tile) -> int64_t {
+    const int64_t block = kPair ? 2 * lane_tile + rank : lane_tile;
+    return block * kLanes < a.lane.rows ? block : 0;
+  };
+  const bool issues = !kPair || rank == 0;
+  auto lane_block = [&](int lane_tile) { return kPair ? 2 * lane_tile + rank : lane_tile; };  // of 128 lanes
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::kStages; ++s) {
       barrier_init(&h.full[s], 1);
       barrier_init(&h.empty[s], 1);
+      barrier_init(&h.peer_full[s], 1);
     }
     for (int s = 0; s < 2; ++s) {
       barrier_init(&h.sum_full[s], 1);
-      barrier_init(&h.sum_empty[s], S::kOutWarps);
+      barrier_init(&h.sum_empty[s], S::kOutWarps * (kPair ? 2 : 1));
     }
     barrier_init(&h.drained, 1);
     h.aborted = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 1) tmem_alloc(&h.tmem, kTmemColumns);
+  if (warp == 1) tmem_alloc<kPair>(&h.tmem, kTmemColumns);
   tcgen05_fence_before();
   __syncthreads();
+  if (kPair) cluster_barrier();  // the other CTA's barriers are ready
   tcgen05_fence_after();
   const uint32_t tmem = h.tmem;
 
@@ -164,8 +183,8 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
         for (int s = 0; s < ahead; ++s) {
           uint8_t* to = stages + s * S::kStageBytes;
           barrier_arrive_expect(&h.full[s], S::kStageBytes);
-          load_box(to, &lane_map, (k0 + s) * kTileBytes, lt * kLanes, &h.full[s]);
-          load_bytes(to + kLaneBytes + kColumns * kTileBytes, a.lane.block_scales + (lt * a.scale_tiles + (k0 + s) * 4) * 512,
+          load_box(to, &lane_map, (k0 + s) * kTileBytes, lane_block(lt) * kLanes, &h.full[s]);
+          load_bytes(to + kLaneBytes + S::kColumnBytes, a.lane.block_scales + (lane_scale_block(lt) * a.scale_tiles + (k0 + s) * 4) * 512,
                      kScaleBytes, &h.full[s]);
         }
       __syncwarp();
@@ -174,7 +193,7 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
     for (int tile = first; ok && tile < tiles; tile += step) {
       int lt, ct;
       place(a, tile, &lt, &ct);
-      const uint8_t* lane_scales = a.lane.block_scales + lt * a.scale_tiles * 512;
+      const uint8_t* lane_scales = a.lane.block_scales + lane_scale_block(lt) * a.scale_tiles * 512;
       const uint8_t* column_scales[S::kBlocks];
 #pragma unroll
       for (int c = 0; c < S::kBlocks; ++c) {
@@ -192,11 +211,11 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
           uint8_t* to = stages + ring.stage * S::kStageBytes;
           if (n >= ahead) {
             barrier_arrive_expect(full, S::kStageBytes);
-            load_box(to, &lane_map, k * kTileBytes, lt * kLanes, full);
-            load_bytes(to + kLaneBytes + kColumns * kTileBytes, lane_scales + k * kScaleBytes, kScaleBytes, full);
+            load_box(to, &lane_map, k * kTileBytes, lane_block(lt) * kLanes, full);
+            load_bytes(to + kLaneBytes + S::kColumnBytes, lane_scales + k * kScaleBytes, kScaleBytes, full);
           }
-          load_box(to + kLaneBytes, &column_map, k * kTileBytes, ct * kColumns, full);
-          to += kLaneBytes + kColumns * kTileBytes;
+          load_box(to + kLaneBytes, &column_map, k * kTileBytes, ct * kColumns + (kPair ? rank * S::kColumnRows : 0), full);
+          to += kLaneBytes + S::kColumnBytes;
 #pragma unroll
           for (int c = 0; c < S::kBlocks; ++c)
             load_bytes(to + kScaleBytes * (1 + c), column_scales[c] + k * kScaleBytes, kScaleBytes, full);
@@ -209,13 +228,23 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
       for (int u = max(0, n - S::kStages); u < n; ++u)
         for (int i = 0; i < kBarrierPolls && !barrier_try(&h.full[u % S::kStages], (u / S::kStages) & 1); ++i) {
         }
+  } else if (warp == 1 && !issues) {  // the pair's second CTA: its loads are in
+    Ring<S::kStages> ring;
+    bool ok = true;
+    for (int tile = first; ok && tile < tiles; tile += step)
+      for (int k = k0; ok && k < k1; ++k, ring.next()) {
+        ok = barrier_wait(&h.full[ring.stage], ring.round & 1, aborted);
+        if (ok && elect_one()) barrier_arrive_at(&h.peer_full[ring.stage], 0);
+        __syncwarp();
+      }
+    if (!ok && lane == 0) give_up(a, aborted, 5);
   } else if (warp == 1) {  // products
     Ring<S::kStages> ring;
     int t = 0;
     bool ok = true;
     const uint64_t lane_codes = swizzled_descriptor(shared_addr(stages));
     const uint64_t column_codes = swizzled_descriptor(shared_addr(stages + kLaneBytes));
-    const uint64_t scales = plain_descriptor(shared_addr(stages + kLaneBytes + kColumns * kTileBytes));
+    const uint64_t scales = plain_descriptor(shared_addr(stages + kLaneBytes + S::kColumnBytes));
     for (int tile = first; ok && tile < tiles; tile += step, ++t) {
       int lt, ct;
       place(a, tile, &lt, &ct);
@@ -225,10 +254,12 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
         break;
       }
       tcgen05_fence_after();
-      const uint32_t instruction = nvfp4_instruction(min(kColumns, (a.column.rows - ct * kColumns + 15) / 16 * 16));
+      // A pair's halves of B are always whole.
+      const uint32_t instruction = nvfp4_instruction(kPair ? 2 * kLanes : kLanes, kPair ? kColumns : min(kColumns, (a.column.rows - ct * kColumns + 15) / 16 * 16));
       const uint32_t sum = tmem + b * kColumns;
       for (int k = k0; k < k1; ++k, ring.next()) {
-        if (!barrier_wait(&h.full[ring.stage], ring.round & 1, aborted)) {
+        if (!barrier_wait(&h.full[ring.stage], ring.round & 1, aborted) ||
+            (kPair && !barrier_wait(&h.peer_full[ring.stage], ring.round & 1, aborted))) {
           if (lane == 0) give_up(a, aborted, 3);
           ok = false;
           break;
@@ -240,23 +271,23 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
           // In tensor memory four columns per product for the lanes, then four per product and 128 columns.
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            copy_scales(lane_scales + 4 * q, scales + offset + 32 * q);
+            copy_scales<kPair>(lane_scales + 4 * q, scales + offset + 32 * q);
 #pragma unroll
             for (int c = 0; c < S::kBlocks; ++c)
-              copy_scales(column_scales + 4 * (q * S::kBlocks + c), scales + offset + (kScaleBytes >> 4) * (1 + c) + 32 * q);
+              copy_scales<kPair>(column_scales + 4 * (q * S::kBlocks + c), scales + offset + (kScaleBytes >> 4) * (1 + c) + 32 * q);
           }
 #pragma unroll
           for (int q = 0; q < 4; ++q)  // 64 elements are 32 bytes: 2 units of 16
-            nvfp4_mma(sum, lane_codes + offset + 2 * q, column_codes + offset + 2 * q, instruction, lane_scales + 4 * q,
+            nvfp4_mma<kPair>(sum, lane_codes + offset + 2 * q, column_codes + offset + 2 * q, instruction, lane_scales + 4 * q,
                       column_scales + 4 * q * S::kBlocks, k > k0 || q > 0);
-          mma_commit(&h.empty[ring.stage]);
-          if (k == k1 - 1) mma_commit(&h.sum_full[b]);
+          mma_commit<kPair>(&h.empty[ring.stage]);
+          if (k == k1 - 1) mma_commit<kPair>(&h.sum_full[b]);
         }
         __syncwarp();
       }
     }
     if (*aborted) {
-      if (elect_one()) mma_commit(&h.drained);
+      if (elect_one()) mma_commit<kPair>(&h.drained);
       for (int i = 0; i < kBarrierPolls && !barrier_try(&h.drained, 0); ++i) {
       }
     }
@@ -280,7 +311,7 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
         }
         asm volatile("bar.sync 1, %0;" ::"n"(32 * S::kOutWarps) : "memory");
       }
-      const int64_t row = static_cast<int64_t>(lt) * kLanes + quarter * 32 + lane;
+      const int64_t row = static_cast<int64_t>(lane_block(lt)) * kLanes + quarter * 32 + lane;
       const bool in = row < a.lane.rows;
       const float row_scale = in ? __ldg(a.lane.scale + (a.lane.per_row ? row : 0)) : 0.0f;
       const float row_bias = in && a.lane.bias ? __ldg(a.lane.bias + row) : 0.0f;
@@ -301,7 +332,10 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
       for (int c = 0; c < S::kOutColumns / 16; ++c) tmem_loaded(v[c]);
       tcgen05_fence_before();
       __syncwarp();
-      if (lane == 0) barrier_arrive(&h.sum_empty[b]);
+      if (lane == 0) {
+        if (kPair) barrier_arrive_at(&h.sum_empty[b], 0);
+        else barrier_arrive(&h.sum_empty[b]);
+      }
       if (a.split > 1) {
         float* partial = reinterpret_cast<float*>(stages) + part * kLanes + quarter * 32 + lane;  // [column][lane]
 #pragma unroll
@@ -324,8 +358,10 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
   }
   tcgen05_fence_before();
   __syncthreads();
-  if (a.split > 1) {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (kPair) {
+    cluster_barrier();  // neither CTA goes while the other may still arrive on its barriers or use its memory
+  } else if (a.split > 1) {
+    cluster_barrier();
     int lt, ct;
     place(a, first, &lt, &ct);
     const int64_t column0 = static_cast<int64_t>(ct) * kColumns;
@@ -356,9 +392,9 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
                    a.column.bias ? __ldg(a.column.bias + column0 + c) : row_bias));
       }
     }
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    cluster_barrier();
   }
-  if (warp == 1) tmem_free(tmem, kTmemColumns);
+  if (warp == 1) tmem_free<kPair>(tmem, kTmemColumns);
 }
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -388,34 +424,36 @@ bool map_codes(const Nvfp4& m, int rows, CUtensorMap* map) {
                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename O, int kColumns>
+template <typename O, int kColumns, bool kPair = false>
 cudaError_t launch(const Nvfp4& lane, const Nvfp4& column, ProductArgs a, int sm_count, cudaStream_t stream) {
-  using S = Shape<kColumns>;
-  a.lane_tiles = (a.lane.rows + kLanes - 1) / kLanes;
+  using S = Shape<kColumns, kPair>;
+  const int lanes = kPair ? 2 * kLanes : kLanes;
+  a.lane_tiles = (a.lane.rows + lanes - 1) / lanes;
   a.column_tiles = (a.column.rows + kColumns - 1) / kColumns;
   const int64_t tiles = static_cast<int64_t>(a.lane_tiles) * a.column_tiles;
   if (tiles > 0x3fffffff) return cudaErrorInvalidConfiguration;
   a.split = 1;
-  while (a.split < 8 && tiles * a.split * 2 <= sm_count && a.k_tiles >= a.split * 2) a.split *= 2;
+  while (!kPair && a.split < 8 && tiles * a.split * 2 <= sm_count && a.k_tiles >= a.split * 2) a.split *= 2;
+  const int group = kPair ? 2 : a.split;
   CUtensorMap lane_map, column_map;
-  if (!map_codes(lane, kLanes, &lane_map) || !map_codes(column, kColumns, &column_map)) return cudaErrorInvalidValue;
+  if (!map_codes(lane, kLanes, &lane_map) || !map_codes(column, S::kColumnRows, &column_map)) return cudaErrorInvalidValue;
   static SharedLimit limit;
-  const cudaError_t err = limit.raise(product_kernel<O, kColumns>, S::kShared);
+  const cudaError_t err = limit.raise(product_kernel<O, kColumns, kPair>, S::kShared);
   if (err != cudaSuccess) return err;
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3(static_cast<unsigned>(a.split > 1 ? tiles * a.split : std::min<int64_t>(tiles, sm_count)));
+  config.gridDim = dim3(static_cast<unsigned>(a.split > 1 ? tiles * a.split : std::min<int64_t>(tiles, sm_count / group) * group));
   config.blockDim = dim3(S::kThreads);
   config.dynamicSmemBytes = S::kShared;
   config.stream = stream;
   // The kernel may start while the one ahead of it in the stream ends; it waits before it reads (grid_wait).
   cudaLaunchAttribute attributes[2]{};
   attributes[0].id = cudaLaunchAttributeClusterDimension;
-  attributes[0].val.clusterDim = {static_cast<unsigned>(a.split), 1, 1};
+  attributes[0].val.clusterDim = {static_cast<unsigned>(group), 1, 1};
   attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attributes[1].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attributes;
   config.numAttrs = 2;
-  return cudaLaunchKernelEx(&config, product_kernel<O, kColumns>, lane_map, column_map, a);
+  return cudaLaunchKernelEx(&config, product_kernel<O, kColumns, kPair>, lane_map, column_map, a);
 }
 
 }  // namespace
@@ -447,6 +485,9 @@ cudaError_t launch_nvfp4_product(const Nvfp4& a, const Nvfp4& b, const float* bi
     if (y.rows <= 32) return launch<O, 32>(x, y, args, info.sm_count, stream);
     if (y.rows <= 64) return launch<O, 64>(x, y, args, info.sm_count, stream);
     if (y.rows <= 128) return launch<O, 128>(x, y, args, info.sm_count, stream);
+    // Pairs where their tiles fill the GPU and the last one along the columns is not mostly empty.
+    const int64_t across = (y.rows + 255) / 256, pairs = (x.rows + 255) / 256 * across;
+    if (pairs * 2 >= info.sm_count && across * 256 * 7 <= y.rows * 8) return launch<O, 256, true>(x, y, args, info.sm_count, stream);
     return launch<O, 256>(x, y, args, info.sm_count, stream);
   });
 }

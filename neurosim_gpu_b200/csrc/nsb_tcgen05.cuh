@@ -46,6 +46,19 @@ __device__ __forceinline__ bool barrier_try(uint64_t* bar, uint32_t parity) {
   return done != 0;
 }
 
+// Arrives on the barrier that lies at `bar` in the shared memory of the cluster's CTA `rank`.  What it
+// tells of are copies and tensor-core work, which complete on barriers of their own before: no fence for
+// plain memory accesses (release.cluster), which takes the relay of a pair about a microsecond.
+__device__ __forceinline__ void barrier_arrive_at(uint64_t* bar, int rank) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(shared_addr(bar)), "r"(rank));
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
+}
+
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 // Polls before a wait gives up (tens of milliseconds at the least).
 constexpr int kBarrierPolls = 1 << 22;
 
@@ -81,14 +94,22 @@ __device__ __forceinline__ void load_bytes(void* to, const void* from, uint32_t 
 // ---------------------------------------------------------------------------
 // Tensor memory: 128 lanes x 512 columns of 32 bits; an address is lane << 16 | column.
 // ---------------------------------------------------------------------------
-// By one whole warp, which also frees it.  The address lands in *slot (shared memory).
+// By one whole warp (kPair: of each of the two CTAs), which also frees it.  The address lands in *slot (shared memory).
+template <bool kPair>
 __device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t columns) {
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_addr(slot)), "r"(columns) : "memory");
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  if constexpr (kPair) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_addr(slot)), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_addr(slot)), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
 }
 
+template <bool kPair>
 __device__ __forceinline__ void tmem_free(uint32_t address, uint32_t columns) {
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(address), "r"(columns));
+  if constexpr (kPair) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(address), "r"(columns));
+  else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(address), "r"(columns));
 }
 
 __device__ __forceinline__ void tcgen05_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -126,30 +147,50 @@ __device__ __forceinline__ uint64_t plain_descriptor(uint32_t address) {
 // ---------------------------------------------------------------------------
 // Block-scaled products of E2M1 operands with a UE4M3 scale per 16 elements
 // ---------------------------------------------------------------------------
-// 512 bytes of scales (32 rows of 16 bytes) to 4 columns, in each of the four 32-lane quarters.
-// Ordered before the products that the same thread issues after it.
+// A pair (kPair) is a cluster of two CTAs whose tensor cores work on one product: its first CTA issues for
+// both.  Each holds its half of the lanes and sums, its half of B's rows, and the scales of its lanes and
+// of all of B, at the same places.
+
+// 512 bytes of scales (32 rows of 16 bytes) to 4 columns, in each of the four 32-lane quarters (of both
+// CTAs, from the shared memory of each).  Ordered before the products that the same thread issues after it.
+template <bool kPair>
 __device__ __forceinline__ void copy_scales(uint32_t tmem, uint64_t descriptor) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(descriptor) : "memory");
+  if constexpr (kPair) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(descriptor) : "memory");
+  else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(descriptor) : "memory");
 }
 
-// The instruction descriptor: E2M1 x E2M1, UE4M3 scales, M = 128 lanes, N columns, both operands K-major.
-__device__ __forceinline__ uint32_t nvfp4_instruction(int n) {
-  return (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | ((128u >> 4) << 24);
+// The instruction descriptor: E2M1 x E2M1, UE4M3 scales, M lanes (128, of a pair 256), N columns, both operands K-major.
+__device__ __forceinline__ uint32_t nvfp4_instruction(int m, int n) {
+  return (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
-// One thread: D[128, n] (+)= A[128, 64] B[n, 64]^T with the scales at scale_a / scale_b in tensor memory.
+// One thread: D[m, n] (+)= A[m, 64] B[n, 64]^T with the scales at scale_a / scale_b in tensor memory.
+template <bool kPair>
 __device__ __forceinline__ void nvfp4_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t instruction, uint32_t scale_a,
                                           uint32_t scale_b, bool accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(instruction), "r"(scale_a), "r"(scale_b), "r"(accumulate ? 1u : 0u)
-      : "memory");
+  if constexpr (kPair)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(instruction), "r"(scale_a), "r"(scale_b), "r"(accumulate ? 1u : 0u)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(instruction), "r"(scale_a), "r"(scale_b), "r"(accumulate ? 1u : 0u)
+        : "memory");
 }
 
-// Arrives on `bar` once all tcgen05 work that this thread has issued is complete.
+// Arrives on `bar` (of a pair: in both CTAs) once all tcgen05 work that this thread has issued is complete.
+template <bool kPair>
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(shared_addr(bar)) : "memory");
+  if constexpr (kPair)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(shared_addr(bar)),
+                 "h"(static_cast<uint16_t>(3))
+                 : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(shared_addr(bar)) : "memory");
 }
 
 }  // namespace nsb

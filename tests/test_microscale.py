@@ -216,7 +216,7 @@ def test_values_that_are_not_finite_stay_visible(value):
 
 PRODUCTS = [(1, 1, 1), (1, 1000, 16), (1, 129, 4096), (2, 8, 17), (3, 257, 1000), (8, 1001, 5000), (16, 128, 64), (17, 300, 255),
             (33, 100, 256), (64, 131, 257), (127, 129, 512), (128, 128, 768), (129, 257, 63), (130, 2, 320), (255, 640, 1024),
-            (256, 256, 2048), (257, 513, 300), (300, 77, 4104), (520, 1030, 272), (1025, 96, 1600)]
+            (256, 256, 2048), (257, 513, 300), (300, 77, 4104), (520, 1030, 272), (1025, 96, 1600), (2048, 2560, 520), (2300, 2420, 300), (2304, 20_000, 64)]
 
 
 def exact_operand(rows, columns, seed):
