@@ -620,6 +620,23 @@ NSB_API int nsb_nvfp4_readout(const nsb_matrix* state, const nsb_nvfp4* weight, 
                               const nsb_matrix* out, void* workspace, size_t workspace_bytes,
                               int* status, void* stream);
 
+/* A training step of a readout y = Q(x) Q(w)^T + b with floating-point weights.  Forward: states packed
+ * by rows, weights with one scale; largest[0], largest[1] (device) receive the largest |x| and |w|, which
+ * the backward call takes.  Backward, straight through the packing, each product on operands packed along
+ * its own sum: dx = Q(dy) Q(w^T)^T (rows; one scale), dw = Q(dy^T) Q(x^T)^T (one scale each), db = column
+ * sums of dy; a gradient whose pointer is NULL is not computed.  The same as the calls above one by one.
+ * Workspace of both: 16-byte aligned, contents need not be initialised. */
+NSB_API size_t nsb_nvfp4_train_workspace_size(int64_t rows, int64_t cols, int64_t outputs);
+NSB_API int nsb_nvfp4_train_forward(const nsb_matrix* state, const nsb_matrix* weight,
+                                    const float* bias, const nsb_matrix* out, float* largest,
+                                    void* workspace, size_t workspace_bytes, int* status,
+                                    void* stream);
+NSB_API int nsb_nvfp4_train_backward(const nsb_matrix* state, const nsb_matrix* weight,
+                                     const nsb_matrix* grad, const float* largest,
+                                     const nsb_matrix* state_grad, const nsb_matrix* weight_grad,
+                                     float* bias_grad, void* workspace, size_t workspace_bytes,
+                                     int* status, void* stream);
+
 /* out[c] = sum of column c of `value` (float32, in a fixed order): the gradient of a bias. */
 NSB_API size_t nsb_column_sums_workspace_size(int64_t rows, int64_t cols);
 NSB_API int nsb_column_sums(const nsb_matrix* value, float* out, void* workspace,

@@ -2,6 +2,8 @@
 //
 // As in capi.cu, arguments are checked completely before anything is enqueued; a failed check
 // returns a negative status and leaves a message for nsb_last_error().  Nothing here throws.
+#include <algorithm>
+
 #include "nsb_tokens.h"
 
 namespace {
@@ -52,6 +54,24 @@ bool check_workspace(const void* workspace, size_t have, size_t need, size_t ali
 
 int done(cudaError_t err, const char* where) {
   return err == cudaSuccess ? NSB_OK : nsb::set_cuda_error(err, where);
+}
+
+// A packed matrix in a workspace; moves `at` past it.
+nsb::Nvfp4 carve(uint8_t** at, int64_t rows, int64_t cols, bool per_row) {
+  const int64_t pitch = (cols + 31) / 32 * 16, scales = (rows + 127) / 128 * ((cols + 255) / 256) * 2048;
+  uint8_t* bytes = *at;
+  *at += (rows * pitch + scales + 4 * rows + 255) / 256 * 256;
+  return {rows, cols, bytes, pitch, bytes + rows * pitch, reinterpret_cast<float*>(bytes + rows * pitch + scales), per_row};
+}
+
+size_t packed_bytes(int64_t rows, int64_t cols) {
+  uint8_t* at = nullptr;
+  carve(&at, rows, cols, true);
+  return reinterpret_cast<uintptr_t>(at);
+}
+
+bool sizes_ok(int64_t rows, int64_t cols, int64_t outputs) {
+  return rows >= 1 && cols >= 1 && outputs >= 1 && rows < kMost && cols < kMost && outputs < kMost;
 }
 
 }  // namespace
@@ -150,9 +170,7 @@ int nsb_nvfp4_product(const nsb_nvfp4* a, const nsb_nvfp4* b, const float* bias,
 }
 
 size_t nsb_nvfp4_readout_workspace_size(int64_t rows, int64_t cols) {
-  if (rows < 1 || cols < 1 || rows >= kMost || cols >= kMost) return 0;
-  const int64_t codes = rows * ((cols + 31) / 32 * 16), scales = (rows + 127) / 128 * ((cols + 255) / 256) * 2048;
-  return static_cast<size_t>(codes + scales + 4 * rows);
+  return sizes_ok(rows, cols, 1) ? packed_bytes(rows, cols) : 0;
 }
 
 int nsb_nvfp4_readout(const nsb_matrix* state, const nsb_nvfp4* weight, const float* bias, const nsb_matrix* out,
@@ -170,11 +188,84 @@ int nsb_nvfp4_readout(const nsb_matrix* state, const nsb_nvfp4* weight, const fl
   nsb::set_error(NSB_OK, "");
   if (x.rows == 0) return NSB_OK;
   auto* bytes = static_cast<uint8_t*>(workspace);
-  const int64_t pitch = (x.cols + 31) / 32 * 16, scales = (x.rows + 127) / 128 * ((x.cols + 255) / 256) * 2048;
-  const nsb::Nvfp4 q{x.rows, x.cols, bytes, pitch, bytes + x.rows * pitch, reinterpret_cast<float*>(bytes + x.rows * pitch + scales), true};
+  const nsb::Nvfp4 q = carve(&bytes, x.rows, x.cols, true);
   const cudaError_t err = nsb::launch_nvfp4_quantize(x, false, q, nullptr, false, nullptr, static_cast<cudaStream_t>(stream));
   if (err != cudaSuccess) return done(err, "nsb_nvfp4_readout launch");
   return done(nsb::launch_nvfp4_product(q, w, bias, o, true, status, static_cast<cudaStream_t>(stream)), "nsb_nvfp4_readout launch");
+}
+
+// Forward: the packed states and weights; backward: the operands of one product at a time, and the sums
+// of the bias; 256 bytes for the largest sizes.
+size_t nsb_nvfp4_train_workspace_size(int64_t rows, int64_t cols, int64_t outputs) {
+  if (!sizes_ok(rows, cols, outputs)) return 0;
+  const size_t forward = packed_bytes(rows, cols) + packed_bytes(outputs, cols);
+  const size_t state = packed_bytes(rows, outputs) + packed_bytes(cols, outputs);
+  const size_t weight = packed_bytes(outputs, rows) + packed_bytes(cols, rows);
+  return 256 + std::max({forward, state, weight, nsb::column_sums_workspace_bytes(rows, outputs)});
+}
+
+int nsb_nvfp4_train_forward(const nsb_matrix* state, const nsb_matrix* weight, const float* bias, const nsb_matrix* out,
+                            float* largest, void* workspace, size_t workspace_bytes, int* status, void* stream) {
+  nsb::Dense x, w, o;
+  if (!check_matrix(state, &x, "states must be a matrix of float32, float16 or bfloat16", "states are required") ||
+      !check_matrix(weight, &w, "weights must be a matrix of float32, float16 or bfloat16", "weights are required") ||
+      !check_matrix(out, &o, "the output must be a matrix of float32, float16 or bfloat16", "the output is required"))
+    return NSB_ERR_ARGUMENT;
+  if (x.cols != w.cols || w.rows < 1 || o.rows != x.rows || o.cols != w.rows)
+    return nsb::set_error(NSB_ERR_ARGUMENT, "states [M, K], weights [N >= 1, K] and output [M, N] do not fit together");
+  if (reinterpret_cast<uintptr_t>(bias) % 4 != 0 || !largest || reinterpret_cast<uintptr_t>(largest) % 4 != 0)
+    return nsb::set_error(NSB_ERR_ARGUMENT, "two words for the largest sizes are required; they and the bias must be 4-byte aligned");
+  if (!check_workspace(workspace, workspace_bytes, nsb_nvfp4_train_workspace_size(x.rows, x.cols, w.rows), 16)) return NSB_ERR_WORKSPACE;
+  nsb::set_error(NSB_OK, "");
+  if (x.rows == 0) return NSB_OK;
+  const auto s = static_cast<cudaStream_t>(stream);
+  auto* most = reinterpret_cast<unsigned int*>(largest);
+  auto* at = static_cast<uint8_t*>(workspace) + 256;
+  const nsb::Nvfp4 qx = carve(&at, x.rows, x.cols, true), qw = carve(&at, w.rows, w.cols, false);
+  cudaError_t err = nsb::launch_nvfp4_quantize(w, false, qw, most + 1, false, nullptr, s);
+  if (err == cudaSuccess) err = nsb::launch_nvfp4_quantize(x, false, qx, most, false, nullptr, s);
+  if (err == cudaSuccess) err = nsb::launch_nvfp4_product(qx, qw, bias, o, true, status, s);
+  return done(err, "nsb_nvfp4_train_forward launch");
+}
+
+int nsb_nvfp4_train_backward(const nsb_matrix* state, const nsb_matrix* weight, const nsb_matrix* grad, const float* largest,
+                             const nsb_matrix* state_grad, const nsb_matrix* weight_grad, float* bias_grad, void* workspace,
+                             size_t workspace_bytes, int* status, void* stream) {
+  nsb::Dense x, w, d, dx, dw;
+  if (!check_matrix(state, &x, "states must be a matrix of float32, float16 or bfloat16", "states are required") ||
+      !check_matrix(weight, &w, "weights must be a matrix of float32, float16 or bfloat16", "weights are required") ||
+      !check_matrix(grad, &d, "the output's gradient must be a matrix of float32, float16 or bfloat16", "the output's gradient is required") ||
+      (state_grad && !check_matrix(state_grad, &dx, "the states' gradient must be a matrix of float32, float16 or bfloat16", "the states' gradient has no data")) ||
+      (weight_grad && !check_matrix(weight_grad, &dw, "the weights' gradient must be a matrix of float32, float16 or bfloat16", "the weights' gradient has no data")))
+    return NSB_ERR_ARGUMENT;
+  if (x.rows < 1 || w.rows < 1 || x.cols != w.cols || d.rows != x.rows || d.cols != w.rows ||
+      (state_grad && (dx.rows != x.rows || dx.cols != x.cols)) || (weight_grad && (dw.rows != w.rows || dw.cols != w.cols)))
+    return nsb::set_error(NSB_ERR_ARGUMENT, "states [M >= 1, K], weights [N >= 1, K], the output's gradient [M, N] and the gradients do not fit together");
+  if (!largest || reinterpret_cast<uintptr_t>(largest) % 4 != 0 || reinterpret_cast<uintptr_t>(bias_grad) % 4 != 0)
+    return nsb::set_error(NSB_ERR_ARGUMENT, "the largest sizes of the forward call are required; they and the bias's gradient must be 4-byte aligned");
+  if (!check_workspace(workspace, workspace_bytes, nsb_nvfp4_train_workspace_size(x.rows, x.cols, w.rows), 16)) return NSB_ERR_WORKSPACE;
+  nsb::set_error(NSB_OK, "");
+  const auto s = static_cast<cudaStream_t>(stream);
+  auto* most = reinterpret_cast<unsigned int*>(const_cast<float*>(largest));
+  auto* grad_most = static_cast<unsigned int*>(workspace);
+  auto* const first = static_cast<uint8_t*>(workspace) + 256;
+  cudaError_t err = cudaSuccess;
+  if (state_grad) {
+    uint8_t* at = first;
+    const nsb::Nvfp4 qd = carve(&at, d.rows, d.cols, true), qw = carve(&at, w.cols, w.rows, false);
+    err = nsb::launch_nvfp4_quantize(w, true, qw, most + 1, true, nullptr, s);
+    if (err == cudaSuccess) err = nsb::launch_nvfp4_quantize(d, false, qd, grad_most, false, nullptr, s);
+    if (err == cudaSuccess) err = nsb::launch_nvfp4_product(qd, qw, nullptr, dx, true, status, s);
+  }
+  if (weight_grad && err == cudaSuccess) {
+    uint8_t* at = first;
+    const nsb::Nvfp4 qd = carve(&at, d.cols, d.rows, false), qx = carve(&at, x.cols, x.rows, false);
+    err = nsb::launch_nvfp4_quantize(d, true, qd, grad_most, state_grad != nullptr, nullptr, s);
+    if (err == cudaSuccess) err = nsb::launch_nvfp4_quantize(x, true, qx, most, true, nullptr, s);
+    if (err == cudaSuccess) err = nsb::launch_nvfp4_product(qd, qx, nullptr, dw, false, status, s);
+  }
+  if (bias_grad && err == cudaSuccess) err = nsb::launch_column_sums(d, bias_grad, first, s);
+  return done(err, "nsb_nvfp4_train_backward launch");
 }
 
 size_t nsb_column_sums_workspace_size(int64_t rows, int64_t cols) {

@@ -94,9 +94,7 @@ def quantize_nvfp4(value: torch.Tensor, *, per: str = "row", transpose: bool = F
     return _quantize(value.detach(), per == "row", transpose)
 
 
-def _quantize(value: torch.Tensor, per_row: bool, transpose: bool, amax: torch.Tensor | None = None,
-              given: bool = False) -> Nvfp4Matrix:
-    """``amax``: a float32 word that receives the largest |value|, or (``given``) holds it already."""
+def _quantize(value: torch.Tensor, per_row: bool, transpose: bool) -> Nvfp4Matrix:
     view = dense_matrix(value, "value")
     rows, columns = (view.cols, view.rows) if transpose else (view.rows, view.cols)
     if view.cols < 1 or columns < 1:
@@ -113,7 +111,7 @@ def _quantize(value: torch.Tensor, per_row: bool, transpose: bool, amax: torch.T
         view.rows, view.cols, int(transpose), count)
     workspace = value.new_empty(size, dtype=torch.uint8) if size else None
     token_call(value, lib.nsb_nvfp4_quantize, ctypes.byref(view), transpose,
-               ctypes.byref(packed._view), None if amax is None else amax.data_ptr(), given,
+               ctypes.byref(packed._view), None, 0,
                workspace.data_ptr() if size else None, size)
     return packed
 
@@ -180,23 +178,12 @@ def _readout(state: torch.Tensor, weight: Nvfp4Matrix, bias: torch.Tensor | None
     _check_bias(bias, n, device)
     out = state.new_empty((rows, n), dtype=dtype)
     result = _Matrix(out.data_ptr(), rows, n, n, VALUE_TYPES[dtype])
-    # Codes, block scales and scale of the states: nsb_nvfp4_readout_workspace_size.
-    size = rows * ((columns + 31) // 32 * 16) + (rows + 127) // 128 * ((columns + 255) // 256) * 2048 + 4 * rows
+    lib = load_library()
+    size = lib.nsb_nvfp4_readout_workspace_size(rows, columns)
     workspace = state.new_empty(size, dtype=torch.uint8)
-    token_call(state, load_library().nsb_nvfp4_readout, ctypes.byref(view), ctypes.byref(weight._view),
+    token_call(state, lib.nsb_nvfp4_readout, ctypes.byref(view), ctypes.byref(weight._view),
                None if bias is None else bias.data_ptr(), ctypes.byref(result), workspace.data_ptr(), size,
                _status_pointer(device))
-    return out
-
-
-def _column_sums(value: torch.Tensor) -> torch.Tensor:
-    view = dense_matrix(value, "value")
-    out = value.new_empty(view.cols, dtype=torch.float32)
-    lib = load_library()
-    size = lib.nsb_column_sums_workspace_size(view.rows, view.cols)
-    workspace = value.new_empty(size, dtype=torch.uint8)
-    token_call(value, lib.nsb_column_sums, ctypes.byref(view), out.data_ptr(),
-               workspace.data_ptr(), size)
     return out
 
 
@@ -206,33 +193,48 @@ class _Readout(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, state, weight, bias, dtype):
-        # The largest sizes of state and weight come with the forward's packing: the backward's needs no pass for them.
-        most = torch.empty(2, device=state.device, dtype=torch.float32)
-        ctx.save_for_backward(state, weight, most)
-        return nvfp4_product(_quantize(state, True, False, most[:1]), _quantize(weight, False, False, most[1:]),
-                             bias=None if bias is None else bias.detach(), dtype=dtype)
+        x, w = dense_matrix(state, "state"), dense_matrix(weight, "weight")
+        device = state.get_device()
+        if weight.get_device() != device or w.rows < 1:
+            raise ValueError("weights must have at least one row and be on the states' device")
+        _check_bias(bias, w.rows, device)
+        out = state.new_empty((x.rows, w.rows), dtype=dtype)
+        largest = state.new_empty(2, dtype=torch.float32)  # of state and weight, for the backward pass
+        ctx.save_for_backward(state, weight, largest)
+        lib = load_library()
+        size = lib.nsb_nvfp4_train_workspace_size(x.rows, x.cols, w.rows)
+        workspace = state.new_empty(size, dtype=torch.uint8)
+        result = _Matrix(out.data_ptr(), x.rows, w.rows, w.rows, VALUE_TYPES[dtype])
+        token_call(out, lib.nsb_nvfp4_train_forward, ctypes.byref(x), ctypes.byref(w),
+                   None if bias is None else bias.data_ptr(), ctypes.byref(result), largest.data_ptr(),
+                   workspace.data_ptr(), size, _status_pointer(device))
+        return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        state, weight, most = ctx.saved_tensors
-        dx = dw = db = None
-        if grad.stride(1) != 1 and grad.shape[1] > 1 or grad.shape[0] > 1 and grad.stride(0) < grad.shape[1]:
+        state, weight, largest = ctx.saved_tensors
+        wants_state, wants_weight, wants_bias, _ = ctx.needs_input_grad
+        if state.shape[0] == 0:
+            return (torch.zeros_like(state) if wants_state else None,
+                    torch.zeros_like(weight) if wants_weight else None,
+                    weight.new_zeros(weight.shape[0], dtype=torch.float32) if wants_bias else None, None)
+        row_stride, stride = grad.stride()
+        if stride != 1 and grad.shape[1] > 1 or row_stride < grad.shape[1] and grad.shape[0] > 1:
             grad = grad.contiguous()  # e.g. the expanded gradient of a sum
-        grad_most = None
-        if ctx.needs_input_grad[0]:
-            if ctx.needs_input_grad[1]:
-                grad_most = torch.empty(1, device=grad.device, dtype=torch.float32)
-            dx = nvfp4_product(_quantize(grad, True, False, grad_most), _quantize(weight, False, True, most[1:], True),
-                               dtype=state.dtype)
-        if ctx.needs_input_grad[1]:
-            if state.shape[0]:
-                dw = nvfp4_product(_quantize(grad, False, True, grad_most, grad_most is not None),
-                                   _quantize(state, False, True, most[:1], True), dtype=weight.dtype)
-            else:
-                dw = torch.zeros_like(weight)
-        if ctx.needs_input_grad[2]:
-            db = _column_sums(grad)
+        x, w, d = dense_matrix(state, "state"), dense_matrix(weight, "weight"), dense_matrix(grad, "grad")
+        dx = state.new_empty((x.rows, x.cols)) if wants_state else None
+        dw = weight.new_empty((w.rows, w.cols)) if wants_weight else None
+        db = weight.new_empty(w.rows, dtype=torch.float32) if wants_bias else None
+        lib = load_library()
+        size = lib.nsb_nvfp4_train_workspace_size(x.rows, x.cols, w.rows)
+        workspace = state.new_empty(size, dtype=torch.uint8)
+        token_call(grad, lib.nsb_nvfp4_train_backward, ctypes.byref(x), ctypes.byref(w), ctypes.byref(d),
+                   largest.data_ptr(),
+                   ctypes.byref(_Matrix(dx.data_ptr(), x.rows, x.cols, x.cols, x.type)) if wants_state else None,
+                   ctypes.byref(_Matrix(dw.data_ptr(), w.rows, w.cols, w.cols, w.type)) if wants_weight else None,
+                   db.data_ptr() if wants_bias else None, workspace.data_ptr(), size,
+                   _status_pointer(state.get_device()))
         return dx, dw, db, None
 
 

@@ -170,7 +170,9 @@ EXPORTED_SYMBOLS = ("nsb_dendritic_step", "nsb_csr_propagate",
                     "nsb_stimulus_gradient_workspace_size", "nsb_stimulus_gradient",
                     "nsb_nvfp4_quantize_workspace_size", "nsb_nvfp4_quantize",
                     "nsb_nvfp4_dequantize", "nsb_nvfp4_product", "nsb_nvfp4_readout_workspace_size",
-                    "nsb_nvfp4_readout", "nsb_column_sums_workspace_size",
+                    "nsb_nvfp4_readout", "nsb_nvfp4_train_workspace_size",
+                    "nsb_nvfp4_train_forward", "nsb_nvfp4_train_backward",
+                    "nsb_column_sums_workspace_size",
                     "nsb_column_sums", "nsb_adjust_logits", "nsb_last_error", "nsb_abi_version")
 
 
@@ -272,6 +274,12 @@ def load_library() -> ctypes.CDLL:
     lib.nsb_nvfp4_readout_workspace_size.argtypes = [i64, i64]
     lib.nsb_nvfp4_readout_workspace_size.restype = size
     lib.nsb_nvfp4_readout.argtypes = [p(_Matrix), p(_Nvfp4), ptr, p(_Matrix), ptr, size, ptr, ptr]
+    lib.nsb_nvfp4_train_workspace_size.argtypes = [i64, i64, i64]
+    lib.nsb_nvfp4_train_workspace_size.restype = size
+    lib.nsb_nvfp4_train_forward.argtypes = [p(_Matrix), p(_Matrix), ptr, p(_Matrix), ptr, ptr, size,
+                                            ptr, ptr]
+    lib.nsb_nvfp4_train_backward.argtypes = [p(_Matrix), p(_Matrix), p(_Matrix), ptr, p(_Matrix),
+                                             p(_Matrix), ptr, ptr, size, ptr, ptr]
     lib.nsb_column_sums_workspace_size.argtypes = [i64, i64]
     lib.nsb_column_sums_workspace_size.restype = size
     lib.nsb_column_sums.argtypes = [p(_Matrix), ptr, ptr, size, ptr]

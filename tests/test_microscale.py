@@ -114,7 +114,7 @@ def test_entry_points_refuse_bad_arguments():
     assert product(a=packed(rows=0, codes=None, scales=None, scale=None),
                    out=native._Matrix(None, 0, 6, 6, 0)) == 0
     state, size = native._Matrix(p, 4, 40, 40, 0), lib.nsb_nvfp4_readout_workspace_size(4, 40)
-    assert size == 4 * 32 + 2048 + 16
+    assert size >= 4 * 32 + 2048 + 16 and lib.nsb_nvfp4_readout_workspace_size(0, 40) == 0
 
     def readout(state=state, weight=packed(rows=6), out=out, workspace=p, size=size, bias=None):
         return lib.nsb_nvfp4_readout(ctypes.byref(state), ctypes.byref(weight), bias, ctypes.byref(out), workspace, size,
@@ -123,6 +123,19 @@ def test_entry_points_refuse_bad_arguments():
     for bad in ({"weight": packed(rows=7)}, {"weight": packed(rows=6, cols=41)}, {"bias": p + 2}, {"state": native._Matrix(p, 5, 40, 40, 0)}):
         assert readout(**bad) == -1, bad
     assert readout(size=size - 1) == -3 and readout(workspace=None) == -3 and readout(workspace=p + 8) == -3
+    weight, grad, train = native._Matrix(p, 6, 40, 40, 0), native._Matrix(p, 4, 6, 6, 0), lib.nsb_nvfp4_train_workspace_size(4, 40, 6)
+    assert train > size and lib.nsb_nvfp4_train_workspace_size(4, 0, 6) == 0
+
+    def forward(weight=weight, out=out, largest=p, size=train):
+        return lib.nsb_nvfp4_train_forward(ctypes.byref(state), ctypes.byref(weight), None, ctypes.byref(out), largest, p, size, None, None)
+
+    def backward(grad=grad, dx=state, dw=weight, largest=p, size=train):
+        return lib.nsb_nvfp4_train_backward(ctypes.byref(state), ctypes.byref(weight), ctypes.byref(grad), largest, ctypes.byref(dx),
+                                            ctypes.byref(dw), None, p, size, None, None)
+
+    assert forward(size=train - 1) == -3 and backward(size=train - 1) == -3
+    assert forward(largest=None) == -1 and backward(largest=None) == -1 and backward(grad=out, dx=out) == -1
+    assert forward(weight=native._Matrix(p, 6, 41, 41, 0)) == -1 and backward(dw=native._Matrix(p, 5, 40, 40, 0)) == -1
     assert lib.nsb_nvfp4_dequantize(ctypes.byref(packed()), ctypes.byref(native._Matrix(p, 4, 41, 41, 0)), None) == -1
     assert lib.nsb_column_sums(ctypes.byref(value), None, p, 10**6, None) == -1
     assert lib.nsb_column_sums(ctypes.byref(value), p, p, 1, None) == -3
