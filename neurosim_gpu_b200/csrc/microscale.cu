@@ -525,14 +525,15 @@ cudaError_t quantize_rows(const Dense& x, const Nvfp4& out, const unsigned int* 
   cudaError_t err = device_info(&info);
   if (err != cudaSuccess) return err;
   const int64_t blocks = block_scale_tiles(x.cols) * 4;
-  // Two or three blocks to a thread (up to four are held); a long row is shared by a cluster while there
-  // are SMs for it, then by up to eight CTAs where four blocks do not hold it, then read twice.
+  // Two blocks to a thread, and up to a quarter more read twice (four in registers leave half the warps);
+  // a long row is shared by a cluster while there are SMs for it, then by up to eight CTAs where four
+  // blocks do not hold it, then read twice.
   int per_row = 4, cluster = 0;
   while (1 << per_row < kRowThreads && blocks > int64_t{3} << per_row) ++per_row;
   while (cluster < 3 && blocks > int64_t{2} << (per_row + cluster) && x.rows << (cluster + 1) <= info.sm_count) ++cluster;
   while (cluster < 3 && blocks > int64_t{4} << (per_row + cluster)) ++cluster;
   if (cluster > 0) per_row = 8;  // a cluster's CTAs are whole
-  const int held = blocks <= int64_t{1} << (per_row + cluster) ? 1 : blocks <= int64_t{2} << (per_row + cluster) ? 2 : 4;
+  const int held = blocks <= int64_t{1} << (per_row + cluster) ? 1 : blocks * 2 <= int64_t{5} << (per_row + cluster) ? 2 : 4;
   const int64_t grid = cluster > 0 ? x.rows << cluster : ((x.rows << per_row) + kRowThreads - 1) / kRowThreads;
   const int64_t fill = x.rows % 128 ? ((blocks + 63) / 64 + (1 << cluster) - 1) >> cluster << cluster : 0;
   if (grid + fill > 0x7fffffff) return cudaErrorInvalidConfiguration;
