@@ -525,7 +525,8 @@ cudaError_t quantize_rows(const Dense& x, const Nvfp4& out, const unsigned int* 
   cudaError_t err = device_info(&info);
   if (err != cudaSuccess) return err;
   const int64_t blocks = block_scale_tiles(x.cols) * 4;
-  // Two blocks to a thread, and up to a quarter more read twice (four in registers leave half the warps);
+  // Two blocks to a thread, and up to a quarter more read twice (four in registers leave half the warps;
+  // off the boundaries, where each takes more registers yet, two: 1,453 x 46,171 float16 101 us against 127);
   // a long row is shared by a cluster while there are SMs for it, then by up to eight CTAs where four
   // blocks do not hold it, then read twice.
   int per_row = 4, cluster = 0;
@@ -533,7 +534,7 @@ cudaError_t quantize_rows(const Dense& x, const Nvfp4& out, const unsigned int* 
   while (cluster < 3 && blocks > int64_t{2} << (per_row + cluster) && x.rows << (cluster + 1) <= info.sm_count) ++cluster;
   while (cluster < 3 && blocks > int64_t{4} << (per_row + cluster)) ++cluster;
   if (cluster > 0) per_row = 8;  // a cluster's CTAs are whole
-  const int held = blocks <= int64_t{1} << (per_row + cluster) ? 1 : blocks * 2 <= int64_t{5} << (per_row + cluster) ? 2 : 4;
+  const int held = blocks <= int64_t{1} << (per_row + cluster) ? 1 : blocks * 2 <= int64_t{5} << (per_row + cluster) || !kVec ? 2 : 4;
   const int64_t grid = cluster > 0 ? x.rows << cluster : ((x.rows << per_row) + kRowThreads - 1) / kRowThreads;
   const int64_t fill = x.rows % 128 ? ((blocks + 63) / 64 + (1 << cluster) - 1) >> cluster << cluster : 0;
   if (grid + fill > 0x7fffffff) return cudaErrorInvalidConfiguration;
