@@ -80,6 +80,11 @@ __device__ __forceinline__ uint32_t remote_load(uint32_t address) {
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(address) : "memory");
   return v;
 }
+__device__ __forceinline__ uint32_t remote_load16(uint32_t address) {
+  unsigned short v;
+  asm volatile("ld.shared::cluster.u16 %0, [%1];" : "=h"(v) : "r"(address) : "memory");
+  return v;
+}
 __device__ __forceinline__ void remote_or(uint32_t address, uint32_t v) {
   asm volatile("red.relaxed.cluster.shared::cluster.or.b32 [%0], %1;" ::"r"(address), "r"(v) : "memory");
 }
@@ -153,13 +158,13 @@ logits_kernel(LogitsArgs a, int ctas, int room) {
   constexpr int kWords = kOwn * threads;
   const int part_vectors = (room < kListed ? kPart : kListed) / P;
   __shared__ uint32_t bits[kHistory ? kWords : 1];    // of the part's tokens: it occurs in the history
-  __shared__ uint32_t before[kHistory ? kWords : 1];  // set bits in the words before
+  __shared__ uint16_t before[kHistory ? kWords : 1];  // set bits in the words before: at most kListed
   extern __shared__ uint32_t counts[];                // per set bit
   // Which 16-bit values of a vector a byte of bits drops, as masks of them.
   constexpr bool kTable = kVec && sizeof(T) == 2;
   __shared__ uint4 masks[kTable ? 256 : 1];
-  T* met = reinterpret_cast<T*>(counts + room);                    // its logit
-  auto* listed = reinterpret_cast<uint16_t*>(met + room);          // its token, less v0, the low 16 bits
+  auto* listed = reinterpret_cast<uint16_t*>(counts + room);          // its token, less v0, the low 16 bits
+  T* met = reinterpret_cast<T*>(listed + (room + 1) / 2 * 2);         // its logit, where the result is written over it
   __shared__ uint32_t scan[32];
   __shared__ Best best_of[32], stream_of[32];
   __shared__ Best cta_best;
@@ -170,7 +175,7 @@ logits_kernel(LogitsArgs a, int ctas, int room) {
   const int vocabulary = static_cast<int>(a.logits.cols);
   const T* in = static_cast<const T*>(a.logits.data) + b * a.logits.stride;
   T* out = static_cast<T*>(a.out.data) + b * a.out.stride;
-  const bool in_place = in == out;
+  const bool in_place = a.logits.data == a.out.data;
   const float* bias = a.bias ? a.bias + b * a.bias_stride : nullptr;
   const int32_t* mask = a.mask ? a.mask + b * a.mask_stride : nullptr;
   const int32_t* history = a.history + b * a.history_stride;
@@ -257,7 +262,7 @@ logits_kernel(LogitsArgs a, int ctas, int room) {
       uint32_t sum = 0;
       for (int i = 0; i < own; ++i) {
         const int w = threadIdx.x * own + i;
-        before[w] = sum;
+        before[w] = static_cast<uint16_t>(sum);
         sum += __popc(bits[w]);
       }
       uint32_t upto = sum;
@@ -271,7 +276,7 @@ logits_kernel(LogitsArgs a, int ctas, int room) {
       const uint32_t one = lane < threads / 32 ? scan[lane] : 0;
       found = __reduce_add_sync(0xffffffffu, one);
       const uint32_t start = upto - sum + __reduce_add_sync(0xffffffffu, lane < warp ? one : 0);
-      for (int i = 0; i < own; ++i) before[threadIdx.x * own + i] += start;
+      for (int i = 0; i < own; ++i) before[threadIdx.x * own + i] += static_cast<uint16_t>(start);
       __syncthreads();
       for (int w = threadIdx.x; w < own * threads; w += threads) {
         uint32_t n = before[w];
@@ -291,7 +296,7 @@ logits_kernel(LogitsArgs a, int ctas, int room) {
           const int w = (place[j] & 0xfffff) >> 5, owner = place[j] >> 20;
           const uint32_t lower = (1u << (place[j] & 31)) - 1u;
           if (together) {
-            const uint32_t n = remote_load(remote_address(before + w, owner)) + __popc(remote_load(remote_address(bits + w, owner)) & lower);
+            const uint32_t n = remote_load16(remote_address(before + w, owner)) + __popc(remote_load(remote_address(bits + w, owner)) & lower);
             remote_add(remote_address(counts + n, owner), 1u);
           } else {
             atomicAdd(counts + before[w] + __popc(bits[w] & lower), 1u);
@@ -441,11 +446,12 @@ cudaError_t adjust_rows(const LogitsArgs& a, cudaStream_t stream) {
   if (a.logits.rows * ctas <= info.sm_count && a.logits.cols >= 4096 * int64_t{ctas}) threads = 1024;
   auto* kernel = threads == 256 ? logits_kernel<T, kVec, kHistory, 256> : logits_kernel<T, kVec, kHistory, 1024>;
   const int room = kHistory ? static_cast<int>(std::min<int64_t>(a.history_length, kListed)) : 0;
-  // A counter, a logit and a place (below 2^16) for each token that may occur.
-  constexpr int kEach = 4 + static_cast<int>(sizeof(T)) + 2;
-  const int shared = room * kEach;
+  // A counter and a place for each token that may occur, and its logit where the result is written over it
+  // (less shared memory leaves more of it to L1, which the shifted vectors of the bias need).
+  constexpr int kMost = kListed * (6 + static_cast<int>(sizeof(T)));
+  const int shared = (room + 1) / 2 * 2 * (6 + (a.logits.data == a.out.data ? static_cast<int>(sizeof(T)) : 0));
   static SharedLimit limits[2];
-  if (kHistory && (err = limits[threads == 256 ? 0 : 1].raise(kernel, kListed * kEach)) != cudaSuccess) return err;
+  if (kHistory && (err = limits[threads == 256 ? 0 : 1].raise(kernel, kMost)) != cudaSuccess) return err;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(static_cast<unsigned>(a.logits.rows * ctas));
   config.blockDim = dim3(threads);

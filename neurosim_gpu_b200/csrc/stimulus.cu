@@ -258,7 +258,7 @@ sort_fill_kernel(const void* tokens, int token_bytes, int64_t n, Sorted s, int p
     uint8_t* row = static_cast<uint8_t*>(out.data) + r * out.stride * bytes_each;
     const int64_t head = min(bytes, static_cast<int64_t>((16 - reinterpret_cast<uintptr_t>(row) % 16) % 16));
     const int64_t vectors = (bytes - head) / 16;
-    for (int64_t i = own; i < vectors; i += stride) reinterpret_cast<uint4*>(row + head)[i] = make_uint4(0, 0, 0, 0);
+    for (int64_t i = own; i < vectors; i += stride) __stcs(reinterpret_cast<uint4*>(row + head) + i, make_uint4(0, 0, 0, 0));
     if (own < head) row[own] = 0;
     if (own < bytes - head - vectors * 16) row[head + vectors * 16 + own] = 0;
   }
