@@ -24,7 +24,7 @@
 //
 // Where there are too few tiles for the GPU, a cluster of 2, 4 or 8 CTAs shares a tile along K: each
 // leaves its float32 partial sums in its shared memory, and each adds a part of the columns of all
-// of them in rank order (deterministic) over distributed shared memory.
+// of them in a fixed order (deterministic) over distributed shared memory.
 #include <cuda.h>
 
 #include <algorithm>
@@ -366,30 +366,47 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
     place(a, first, &lt, &ct);
     const int64_t column0 = static_cast<int64_t>(ct) * kColumns;
     const int columns = static_cast<int>(min(static_cast<int64_t>(kColumns), a.column.rows - column0));
-    const int at = threadIdx.x % kLanes;
+    // A thread adds up L neighbouring lanes of two columns at a time: four of a wide tile, where the other
+    // CTAs' shared memory is read at its rate (512 x 2,048 x 4,096: 10.5 us, single lanes 13.9), one of a narrow
+    // one, where there are threads enough (60 x 1,001 x 4,096: 6.7 us, four lanes 7.4).
+    constexpr int L = kColumns >= 128 ? 4 : 1, kTeams = S::kThreads * L / kLanes;
+    const int team = threadIdx.x * L / kLanes, at = threadIdx.x * L % kLanes;
     const int64_t row = static_cast<int64_t>(lt) * kLanes + at;
-    constexpr int kTeams = S::kThreads / kLanes;
-    if (threadIdx.x < kTeams * kLanes && row < a.lane.rows && !*aborted) {
-      const float row_scale = __ldg(a.lane.scale + (a.lane.per_row ? row : 0));
-      const float row_bias = a.lane.bias ? __ldg(a.lane.bias + row) : 0.0f;
-      for (int c = rank + threadIdx.x / kLanes * a.split; c < columns; c += kTeams * a.split) {
-        float part[8];
+    const int rows = static_cast<int>(max(int64_t{0}, min(static_cast<int64_t>(L), a.lane.rows - row)));
+    if (team < kTeams && rows > 0 && !*aborted) {
+      float row_scale[L], row_bias[L];
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          part[r] = 0.0f;
-          if (r < a.split) {
-            uint32_t remote;
-            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(shared_addr(stages) + (c * kLanes + at) * 4), "r"(r));
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part[r]) : "r"(remote) : "memory");
+      for (int i = 0; i < L; ++i) {
+        const int64_t r = row + min(i, rows - 1);
+        row_scale[i] = __ldg(a.lane.scale + (a.lane.per_row ? r : 0));
+        row_bias[i] = a.lane.bias ? __ldg(a.lane.bias + r) : 0.0f;
+      }
+      const int step = kTeams * a.split;
+      for (int c0 = rank + team * a.split; c0 < columns; c0 += 2 * step) {
+        Pack<float, L> part[2][8];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int c = min(c0 + u * step, kColumns - 1);
+#pragma unroll
+          for (int r = 0; r < 8; ++r)  // its own first, so that the CTAs do not all read the same one
+            if (r < a.split) remote_load(shared_addr(stages) + (c * kLanes + at) * 4, (rank + r) & (a.split - 1), part[u][r].v);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int c = c0 + u * step;
+          if (c >= columns) break;
+          const float scale = __ldg(a.column.scale + (a.column.per_row ? column0 + c : 0));
+          O* to = static_cast<O*>(a.out) + row * a.lane.stride + (column0 + c) * a.column.stride;
+#pragma unroll
+          for (int i = 0; i < L; ++i) {
+            float sum = part[u][0].v[i];
+#pragma unroll
+            for (int r = 1; r < 8; ++r)
+              if (r < a.split) sum += part[u][r].v[i];
+            if (i < rows)
+              to[i * a.lane.stride] = Values<O>::down(scaled(sum, row_scale[i], scale, a.column.bias ? __ldg(a.column.bias + column0 + c) : row_bias[i]));
           }
         }
-        float sum = part[0];
-#pragma unroll
-        for (int r = 1; r < 8; ++r)
-          if (r < a.split) sum += part[r];
-        static_cast<O*>(a.out)[row * a.lane.stride + (column0 + c) * a.column.stride] = Values<O>::down(
-            scaled(sum, row_scale, __ldg(a.column.scale + (a.column.per_row ? column0 + c : 0)),
-                   a.column.bias ? __ldg(a.column.bias + column0 + c) : row_bias));
       }
     }
     cluster_barrier();
@@ -432,14 +449,23 @@ cudaError_t launch(const Nvfp4& lane, const Nvfp4& column, ProductArgs a, int sm
   a.column_tiles = (a.column.rows + kColumns - 1) / kColumns;
   const int64_t tiles = static_cast<int64_t>(a.lane_tiles) * a.column_tiles;
   if (tiles > 0x3fffffff) return cudaErrorInvalidConfiguration;
-  a.split = 1;
-  while (!kPair && a.split < 8 && tiles * a.split * 2 <= sm_count && a.k_tiles >= a.split * 2) a.split *= 2;
-  const int group = kPair ? 2 : a.split;
   CUtensorMap lane_map, column_map;
   if (!map_codes(lane, kLanes, &lane_map) || !map_codes(column, S::kColumnRows, &column_map)) return cudaErrorInvalidValue;
   static SharedLimit limit;
-  const cudaError_t err = limit.raise(product_kernel<O, kColumns, kPair>, S::kShared);
+  cudaError_t err = limit.raise(product_kernel<O, kColumns, kPair>, S::kShared);
   if (err != cudaSuccess) return err;
+  // As many CTAs to a tile as leave every cluster a place at once: 74 clusters of 2, 33 of 4, 15 of 8 (8 x
+  // 1,001 x 50,000: 10.9 us with eight, 46 with one; 16 tiles of 64 x 2,000 x 4,096: 7.7 with four, 12.6 with
+  // eight, one of whose clusters has to wait).
+  static ClusterLimit clusters[3];
+  a.split = 1;
+  for (int i = 0; !kPair && i < 3 && a.k_tiles >= 4 << i; ++i) {
+    int most = 0;
+    if ((err = clusters[i].most(product_kernel<O, kColumns, kPair>, 2 << i, S::kThreads, S::kShared, &most)) != cudaSuccess) return err;
+    if (tiles > most) break;
+    a.split = 2 << i;
+  }
+  const int group = kPair ? 2 : a.split;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(static_cast<unsigned>(a.split > 1 ? tiles * a.split : std::min<int64_t>(tiles, sm_count / group) * group));
   config.blockDim = dim3(S::kThreads);
@@ -469,8 +495,9 @@ cudaError_t launch_nvfp4_product(const Nvfp4& a, const Nvfp4& b, const float* bi
     args.scale_tiles = block_scale_tiles(a.cols);
     args.k_tiles = static_cast<int32_t>((a.cols + 255) / 256);
     args.status = status;
-    // Few rows of b (a narrow readout of many states) go along the columns; else b along the lanes,
-    // where neighbouring lanes write neighbouring outputs.
+    // Few rows of b (a narrow readout of many states) go along the columns (8,192 x 25 x 4,096: 10.3 us against
+    // 20.1 along the lanes; 300 x 25 x 4,096: 6.1 against 10.8); else b along the lanes, where neighbouring
+    // lanes write neighbouring outputs.
     const bool narrow = b.rows <= 128 && b.rows < a.rows;
     args.lane = narrow ? rows : cols;
     args.column = narrow ? cols : rows;
@@ -479,16 +506,16 @@ cudaError_t launch_nvfp4_product(const Nvfp4& a, const Nvfp4& b, const float* bi
     DeviceInfo info;
     const cudaError_t err = device_info(&info);
     if (err != cudaSuccess) return err;
-    // The least tile that holds all columns; beyond 128 the widest one (a tile has to start on a
-    // 128-row tile of block scales).
+    // The least tile that holds all columns (1 x 32,000 x 4,096: 15.3 us with 16 columns, 21.9 with 128;
+    // 60 x 16,000 x 4,096: 10.7 with 64, 14.2 with 128).  Beyond 128 (a tile has to start on a 128-row tile
+    // of block scales) pairs' tiles of 256 lanes x 256 columns, unless all tiles of 128 x 128 run at once
+    // (1,024 x 2,048 x 4,096: 7.9 us, pairs 10.5; 256 x 2,048 x 16,384: 13.4 on four CTAs a tile, pairs 24.4;
+    // 2,048 x 2,048 x 4,096: pairs 11.1, 128 x 128 12.3; 8,192 x 8,192 x 4,096: pairs 109, 128 x 128 143).
     if (y.rows <= 16) return launch<O, 16>(x, y, args, info.sm_count, stream);
     if (y.rows <= 32) return launch<O, 32>(x, y, args, info.sm_count, stream);
     if (y.rows <= 64) return launch<O, 64>(x, y, args, info.sm_count, stream);
-    if (y.rows <= 128) return launch<O, 128>(x, y, args, info.sm_count, stream);
-    // Pairs where their tiles fill the GPU and the last one along the columns is not mostly empty.
-    const int64_t across = (y.rows + 255) / 256, pairs = (x.rows + 255) / 256 * across;
-    if (pairs * 2 >= info.sm_count && across * 256 * 7 <= y.rows * 8) return launch<O, 256, true>(x, y, args, info.sm_count, stream);
-    return launch<O, 256>(x, y, args, info.sm_count, stream);
+    if ((x.rows + 127) / 128 * ((y.rows + 127) / 128) <= info.sm_count || y.rows <= 128) return launch<O, 128>(x, y, args, info.sm_count, stream);
+    return launch<O, 256, true>(x, y, args, info.sm_count, stream);
   });
 }
 

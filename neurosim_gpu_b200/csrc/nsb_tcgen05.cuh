@@ -21,6 +21,20 @@ __device__ __forceinline__ bool elect_one() {
 // Until the kernels ahead in the stream are complete (a launch that may overlap them).
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// One float32, or four, of CTA `rank`'s shared memory in the cluster, where this CTA's `address` would be.
+__device__ __forceinline__ uint32_t remote_address(uint32_t address, int rank) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(address), "r"(rank));
+  return remote;
+}
+__device__ __forceinline__ void remote_load(uint32_t address, int rank, float (&v)[1]) {
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[0]) : "r"(remote_address(address, rank)) : "memory");
+}
+__device__ __forceinline__ void remote_load(uint32_t address, int rank, float (&v)[4]) {
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(remote_address(address, rank)) : "memory");
+}
+
 // ---------------------------------------------------------------------------
 // mbarriers
 // ---------------------------------------------------------------------------

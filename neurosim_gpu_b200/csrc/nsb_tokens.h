@@ -24,6 +24,33 @@ struct SharedLimit {
   }
 };
 
+// How many clusters of a kernel's CTAs run at once on the current device, asked once per device.
+struct ClusterLimit {
+  int known[64] = {};
+  template <typename K>
+  cudaError_t most(K* kernel, int cluster, int threads, int shared, int* clusters) {
+    int device = 0;
+    cudaError_t err = cudaGetDevice(&device);
+    if (err != cudaSuccess) return err;
+    if (known[device & 63] == 0) {
+      cudaLaunchConfig_t config{};
+      config.gridDim = dim3(static_cast<unsigned>(cluster));
+      config.blockDim = dim3(static_cast<unsigned>(threads));
+      config.dynamicSmemBytes = static_cast<size_t>(shared);
+      cudaLaunchAttribute attribute{};
+      attribute.id = cudaLaunchAttributeClusterDimension;
+      attribute.val.clusterDim = {static_cast<unsigned>(cluster), 1, 1};
+      config.attrs = &attribute;
+      config.numAttrs = 1;
+      int found = 0;
+      if ((err = cudaOccupancyMaxActiveClusters(&found, kernel, &config)) != cudaSuccess) return err;
+      known[device & 63] = found;
+    }
+    *clusters = known[device & 63];
+    return cudaSuccess;
+  }
+};
+
 // stimulus.cu
 cudaError_t launch_stimulus_drive(const void* tokens, int token_bytes, int64_t n, const Dense& table,
                                   float scale, const Dense& out, cudaStream_t stream);
