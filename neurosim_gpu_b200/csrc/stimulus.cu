@@ -83,6 +83,7 @@ __device__ __forceinline__ Pack<T, 16 / sizeof(T)> load_anywhere(const T* p, con
 // vector is 16 bytes of the table's type.  kAligned: rows of both matrices start on vectors; else a row
 // is cut where its output reaches a vector's boundary, and the table's values are shifted into place
 // (4,000 x 4,001 bf16: 14.4 us; single columns a warp's width apart 20.0; on vectors 6 would do).
+// Bound by HBM: 160 ids x 166,000 bf16 to f32 23.8 us, 6.7 TB/s with the table's rows counted once.
 template <typename In, typename O, bool kAligned>
 __global__ void __launch_bounds__(kDriveThreads)
 drive_kernel(const void* tokens, int token_bytes, int64_t n, Dense table, float scale, Dense out,
@@ -131,7 +132,8 @@ struct Sorted {
 // Stable least-significant-byte radix sort of the keys min(token, limit) by one cluster.
 // Warp g of the cluster's 256 owns elements [g * span, (g + 1) * span).  Per pass: each warp
 // counts its digits; a scan over (digit, CTA, warp) gives each warp the first slot of each of
-// its digits; the warp walks its elements again in order and places them.
+// its digits; the warp walks its elements again in order and places them.  All latency: 32,768 ids, two
+// passes, 22.8 us; two clusters and more would have to meet in global memory between the passes.
 __device__ void sort_tokens(cg::cluster_group& cluster, const void* tokens, int token_bytes,
                             int64_t n, int64_t limit, const Sorted& s, int passes,
                             uint32_t (*hist)[kDigits], uint32_t* totals, uint32_t* scan, uint32_t* first_of) {
@@ -275,7 +277,8 @@ struct Partials {
 
 // A thread sums 16 bytes' worth of columns: a vector (kAligned: rows of both matrices start on vectors),
 // or single columns kSegmentThreads apart (60,000 tokens x 1,001 bf16: 40 us; cutting vectors out of
-// aligned loads 95: too many selects in front of the sums).
+// aligned loads 95: too many selects in front of the sums).  Bound by HBM where tokens do not repeat much:
+// 32,768 x 2,048 bf16 31.7 us, 4.2 TB/s.
 template <typename In, typename O, bool kAligned>
 __global__ void __launch_bounds__(kSegmentThreads, kAligned ? 8 : 6)
 segment_kernel(const uint32_t* __restrict__ key, const uint32_t* __restrict__ pos, int64_t n,
@@ -354,6 +357,7 @@ segment_kernel(const uint32_t* __restrict__ key, const uint32_t* __restrict__ po
 
 // Tile j joins the run that starts in it and goes on into later tiles.  A short run: each of the CTA's
 // warps takes 128 columns; a long one: the warps share its tiles, and their sums are added in warp order.
+// A chain of dependent loads (keys, then partials): 8.9 us for 32,768 x 2,048.
 template <typename O>
 __global__ void __launch_bounds__(32 * kJoinWarps)
 join_kernel(const uint32_t* __restrict__ key, int64_t n, int tile, float scale, Dense out,

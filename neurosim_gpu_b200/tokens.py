@@ -41,7 +41,7 @@ def generate_tokens(runtime, table: torch.Tensor, readout: Nvfp4Matrix | torch.T
     length = prompt.shape[1]
     with torch.inference_mode():
         history = torch.full((batch, length + steps), -1, device=prompt.device, dtype=torch.int32)
-        history[:, :length] = prompt
+        history[:, :length] = prompt.clamp(-1, 2**31 - 1)  # what no table has stays outside it
         prompts = torch.full((batch,), length, device=prompt.device, dtype=torch.int32)
         answer = torch.empty((batch, steps), device=prompt.device, dtype=torch.int64)
         for at in range(length + steps - 1 if steps else 0):

@@ -212,3 +212,16 @@ def test_strided_rows_in_place_and_graph(dtype):
     a.zero_(), b.zero_()
     graph.replay()
     assert torch.equal(a, want) and torch.equal(b, choice)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocabulary,length", [(2, 131_071, 4096), (2, 200_003, 40_000), (1, 600_000, 5000), (3, 1001, 70_000)])
+def test_long_histories_in_place(dtype, rows, vocabulary, length):
+    logits = (3 * torch.randn(rows, vocabulary, generator=generator(4))).to(dtype)
+    kw = case(rows, vocabulary, length)
+    got, choice = check(logits, dtype, **kw)
+    device = {("prompt_lengths" if k == "prompts" else k): v.cuda() for k, v in kw.items()}
+    x = logits.cuda()
+    again, same = adjust_logits(x, out=x, choose=True, **device)
+    assert again is x and torch.equal(x, got) and torch.equal(same, choice)
