@@ -162,17 +162,32 @@ __device__ void sort_tokens(cg::cluster_group& cluster, const void* tokens, int 
     }
     for (int d = lane; d < kDigits; d += 32) hist[warp][d] = 0;
     __syncwarp();
-    auto count = [&](int64_t i, uint32_t key) {
-      const bool in = i < last;
-      const uint32_t digit = in ? (key >> shift) & (kDigits - 1) : ~0u;
-      const uint32_t same = __match_any_sync(0xffffffffu, digit);
-      if (in && (same & below) == 0) hist[warp][digit] += __popc(same);
+    // The lanes that hold the same digit, of those that hold one.
+    auto equals = [&](bool in, uint32_t key) {
+      uint32_t same = __ballot_sync(0xffffffffu, in);
+#pragma unroll
+      for (int b = 0; b < 8; ++b) {
+        const bool bit = key >> (shift + b) & 1;
+        const uint32_t set = __ballot_sync(0xffffffffu, bit);
+        same &= bit ? set : ~set;
+      }
+      return same;
+    };
+    auto count = [&](bool in, uint32_t key, uint32_t same) {
+      if (in && (same & below) == 0) hist[warp][(key >> shift) & (kDigits - 1)] += __popc(same);
       __syncwarp();
     };
+    uint32_t held_same[kHeld];
 #pragma unroll
-    for (int r = 0; r < kHeld; ++r)
-      if (first + 32 * r < last) count(first + 32 * r + lane, held[r]);
-    for (int64_t i = first + 32 * kHeld; i < last; i += 32) count(i + lane, i + lane < last ? key_of(i + lane) : 0);
+    for (int r = 0; r < kHeld; ++r) {
+      const bool in = first + 32 * r + lane < last;
+      if (first + 32 * r < last) count(in, held[r], held_same[r] = equals(in, held[r]));
+    }
+    for (int64_t i = first + 32 * kHeld; i < last; i += 32) {
+      const bool in = i + lane < last;
+      const uint32_t key = in ? key_of(i + lane) : 0;
+      count(in, key, equals(in, key));
+    }
     __syncthreads();
     if (threadIdx.x < kDigits) {
       uint32_t c[kSortWarps], sum = 0;
@@ -214,10 +229,8 @@ __device__ void sort_tokens(cg::cluster_group& cluster, const void* tokens, int 
     __syncthreads();
     uint32_t* key_out = s.key[pass & 1];
     uint32_t* pos_out = s.pos[pass & 1];
-    auto place = [&](int64_t i, uint32_t key, uint32_t pos) {
-      const bool in = i < last;
-      const uint32_t digit = in ? (key >> shift) & (kDigits - 1) : ~0u;
-      const uint32_t same = __match_any_sync(0xffffffffu, digit);
+    auto place = [&](bool in, uint32_t key, uint32_t pos, uint32_t same) {
+      const uint32_t digit = (key >> shift) & (kDigits - 1);
       uint32_t slot = 0;
       if (in) slot = first_of[digit] + hist[warp][digit] + __popc(same & below);
       __syncwarp();
@@ -230,10 +243,11 @@ __device__ void sort_tokens(cg::cluster_group& cluster, const void* tokens, int 
     };
 #pragma unroll
     for (int r = 0; r < kHeld; ++r)
-      if (first + 32 * r < last) place(first + 32 * r + lane, held[r], held_pos[r]);
+      if (first + 32 * r < last) place(first + 32 * r + lane < last, held[r], held_pos[r], held_same[r]);
     for (int64_t i = first + 32 * kHeld; i < last; i += 32) {
       const bool in = i + lane < last;
-      place(i + lane, in ? key_of(i + lane) : 0, in ? pos_of(i + lane) : 0);
+      const uint32_t key = in ? key_of(i + lane) : 0;
+      place(in, key, in ? pos_of(i + lane) : 0, equals(in, key));
     }
     cluster.sync();  // also orders this pass's keys in global memory before the next pass reads them
   }

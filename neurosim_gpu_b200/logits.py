@@ -13,6 +13,9 @@ import torch
 from .native import _Logits, _Matrix, _RowValues, dense_matrix, load_library, token_call
 
 
+_NONE = (None, 0)
+
+
 def _row_values(value: float | torch.Tensor, name: str, rows: int, device: torch.device) -> _RowValues:
     if not isinstance(value, torch.Tensor):
         return _RowValues(None, 0, float(value))
@@ -66,35 +69,33 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
     view = dense_matrix(logits, "logits")
     rows, vocabulary = view.rows, view.cols
     device = logits.device
-    args = _Logits(view)
     if out is None:
         out = logits.new_empty((rows, vocabulary))
-        args.out = _Matrix(out.data_ptr(), rows, vocabulary, vocabulary, view.type)
+        result = _Matrix(out.data_ptr(), rows, vocabulary, vocabulary, view.type)
+    elif out is logits:
+        result = view
     elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != device:
         raise ValueError("out must have the logits' shape, dtype and device")
     else:
-        args.out = view if out is logits else dense_matrix(out, "out")
+        result = dense_matrix(out, "out")
+    past, length, stride = None, 0, 0
     if history is not None:
         if (history.dtype != torch.int32 or history.device != device or history.dim() != 2
                 or history.shape[0] != rows or (history.shape[1] > 1 and history.stride(1) != 1)):
             raise ValueError("history must be int32 [B, L] with contiguous rows")
-        args.history = history.data_ptr()
-        args.history_length, args.history_stride = history.shape[1], history.stride(0)
+        past, length, stride = history.data_ptr(), history.shape[1], history.stride(0)
     elif lengths is not None or prompt_lengths is not None:
         raise ValueError("lengths need a history")
-    if lengths is not None:
-        args.lengths = _lengths(lengths, "lengths", rows, device)
-    if prompt_lengths is not None:
-        args.prompt_lengths = _lengths(prompt_lengths, "prompt_lengths", rows, device)
-    args.repetition = _row_values(repetition, "repetition", rows, device)
-    args.presence = _row_values(presence, "presence", rows, device)
-    args.frequency = _row_values(frequency, "frequency", rows, device)
-    if bias is not None:
-        args.bias, args.bias_stride = _broadcast(bias, "bias", torch.float32, rows, vocabulary, device)
-    if mask is not None:
-        args.mask, args.mask_stride = _broadcast(mask, "mask", torch.int32, rows, (vocabulary + 31) // 32, device)
     choice = logits.new_empty(rows, dtype=torch.int64) if choose else None
-    if choose:
-        args.choice = choice.data_ptr()
+    args = _Logits(
+        view, result, past, length, stride,
+        None if lengths is None else _lengths(lengths, "lengths", rows, device),
+        None if prompt_lengths is None else _lengths(prompt_lengths, "prompt_lengths", rows, device),
+        _row_values(repetition, "repetition", rows, device),
+        _row_values(presence, "presence", rows, device),
+        _row_values(frequency, "frequency", rows, device),
+        *(_NONE if bias is None else _broadcast(bias, "bias", torch.float32, rows, vocabulary, device)),
+        *(_NONE if mask is None else _broadcast(mask, "mask", torch.int32, rows, (vocabulary + 31) // 32, device)),
+        choice.data_ptr() if choose else None)
     token_call(logits, load_library().nsb_adjust_logits, ctypes.byref(args))
     return (out, choice) if choose else out

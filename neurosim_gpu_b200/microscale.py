@@ -58,6 +58,16 @@ class Nvfp4Matrix:
         self._view = _Nvfp4(rows, columns, codes.data_ptr(), shape[1], block_scales.data_ptr(),
                             scale.data_ptr(), count)
 
+    @classmethod
+    def _own(cls, codes: torch.Tensor, block_scales: torch.Tensor, scale: torch.Tensor, rows: int,
+             columns: int, count: int) -> "Nvfp4Matrix":
+        """Of tensors made for it: nothing to check."""
+        self = cls.__new__(cls)
+        self.codes, self.block_scales, self.scale, self.columns = codes, block_scales, scale, columns
+        self._view = _Nvfp4(rows, columns, codes.data_ptr(), (columns + 31) // 32 * 16,
+                            block_scales.data_ptr(), scale.data_ptr(), count)
+        return self
+
     @property
     def rows(self) -> int:
         return self.codes.shape[0]
@@ -91,7 +101,7 @@ def quantize_nvfp4(value: torch.Tensor, *, per: str = "row", transpose: bool = F
     """
     if per not in ("row", "tensor"):
         raise ValueError("per must be 'row' or 'tensor'")
-    return _quantize(value.detach(), per == "row", transpose)
+    return _quantize(value.detach() if value.requires_grad else value, per == "row", transpose)
 
 
 def _quantize(value: torch.Tensor, per_row: bool, transpose: bool) -> Nvfp4Matrix:
@@ -104,7 +114,7 @@ def _quantize(value: torch.Tensor, per_row: bool, transpose: bool) -> Nvfp4Matri
     count = rows if per_row else 1
     # A tensor without rows has the scale of zeros.
     scale = value.new_empty(count, dtype=torch.float32) if rows else value.new_ones(count, dtype=torch.float32)
-    packed = Nvfp4Matrix(codes, scales, scale, columns)
+    packed = Nvfp4Matrix._own(codes, scales, scale, rows, columns, count)
     lib = load_library()
     # A row's own scale needs no workspace; see nsb_nvfp4_quantize_workspace_size.
     size = 0 if per_row and not transpose else lib.nsb_nvfp4_quantize_workspace_size(
