@@ -125,9 +125,13 @@ drive_kernel(const void* tokens, int token_bytes, int64_t n, Dense table, float 
 
 // Workspace: keys and positions, two buffers each, then the partial rows.
 struct Sorted {
-  uint32_t* key[2];
-  uint32_t* pos[2];
+  uint2* pair[2];  // key and position
 };
+
+// Elements of a warp.
+__host__ __device__ inline int64_t sort_span(int64_t n) {
+  return ((n + kSortCtas * kSortWarps - 1) / (kSortCtas * kSortWarps) + 31) / 32 * 32;
+}
 
 // Stable least-significant-byte radix sort of the keys min(token, limit) by one cluster.
 // Warp g of the cluster's 256 owns elements [g * span, (g + 1) * span).  Per pass: each warp
@@ -136,29 +140,28 @@ struct Sorted {
 // passes, 22.8 us; two clusters and more would have to meet in global memory between the passes.
 __device__ void sort_tokens(cg::cluster_group& cluster, const void* tokens, int token_bytes,
                             int64_t n, int64_t limit, const Sorted& s, int passes,
-                            uint32_t (*hist)[kDigits], uint32_t* totals, uint32_t* scan, uint32_t* first_of) {
+                            uint32_t (*hist)[kDigits], uint32_t* totals, uint2* scan, uint2* first_of, uint2* local) {
   const int rank = static_cast<int>(cluster.block_rank());
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t span = ((n + kSortCtas * kSortWarps - 1) / (kSortCtas * kSortWarps) + 31) / 32 * 32;
+  const int64_t span = sort_span(n);
+  const bool staged = span <= 32 * kHeld;
   const int64_t first = (rank * kSortWarps + warp) * span;
   const int64_t last = min(n, first + span);
   const uint32_t below = (1u << lane) - 1u;
   for (int pass = 0; pass < passes; ++pass) {
     const int shift = 8 * pass;
     // L1 is not coherent between SMs: the other CTAs' keys of the last pass are read from L2.
-    auto key_of = [&](int64_t i) -> uint32_t {
-      if (pass > 0) return __ldcg(s.key[(pass - 1) & 1] + i);
+    auto pair_of = [&](int64_t i) -> uint2 {
+      if (pass > 0) return __ldcg(s.pair[(pass - 1) & 1] + i);
       const int64_t token = token_at(tokens, token_bytes, i);
-      return static_cast<uint32_t>(token < 0 || token >= limit ? limit : token);
+      return make_uint2(static_cast<uint32_t>(token < 0 || token >= limit ? limit : token), static_cast<uint32_t>(i));
     };
-    auto pos_of = [&](int64_t i) { return pass > 0 ? __ldcg(s.pos[(pass - 1) & 1] + i) : static_cast<uint32_t>(i); };
     // The first kHeld rounds of 32 elements stay in registers for both walks.
-    uint32_t held[kHeld], held_pos[kHeld];
+    uint2 held[kHeld];
 #pragma unroll
     for (int r = 0; r < kHeld; ++r) {
       const int64_t i = first + 32 * r + lane;
-      held[r] = i < last ? key_of(i) : 0;
-      held_pos[r] = i < last ? pos_of(i) : 0;
+      held[r] = i < last ? pair_of(i) : make_uint2(0, 0);
     }
     for (int d = lane; d < kDigits; d += 32) hist[warp][d] = 0;
     __syncwarp();
@@ -181,11 +184,11 @@ __device__ void sort_tokens(cg::cluster_group& cluster, const void* tokens, int 
 #pragma unroll
     for (int r = 0; r < kHeld; ++r) {
       const bool in = first + 32 * r + lane < last;
-      if (first + 32 * r < last) count(in, held[r], held_same[r] = equals(in, held[r]));
+      if (first + 32 * r < last) count(in, held[r].x, held_same[r] = equals(in, held[r].x));
     }
     for (int64_t i = first + 32 * kHeld; i < last; i += 32) {
       const bool in = i + lane < last;
-      const uint32_t key = in ? key_of(i + lane) : 0;
+      const uint32_t key = in ? pair_of(i + lane).x : 0;
       count(in, key, equals(in, key));
     }
     __syncthreads();
@@ -201,7 +204,7 @@ __device__ void sort_tokens(cg::cluster_group& cluster, const void* tokens, int 
       totals[threadIdx.x] = sum;
     }
     cluster.sync();
-    uint32_t before = 0, all = 0;
+    uint32_t before = 0, all = 0, here = 0;
     if (threadIdx.x < kDigits) {
       uint32_t x[kSortCtas];
 #pragma unroll
@@ -211,43 +214,58 @@ __device__ void sort_tokens(cg::cluster_group& cluster, const void* tokens, int 
         before += c < rank ? x[c] : 0;
         all += x[c];
       }
-      // Exclusive scan over the digits: within the warp, then over the 8 warps that hold them.
-      uint32_t sum = all;
+      // Exclusive scans over the digits, of the cluster and of the CTA: within the warp, then over the 8
+      // warps that hold them.
+      here = totals[threadIdx.x];
+      uint32_t sum = all, own = here;
       for (int off = 1; off < 32; off <<= 1) {
-        const uint32_t up = __shfl_up_sync(0xffffffffu, sum, off);
-        if (lane >= off) sum += up;
+        const uint32_t up = __shfl_up_sync(0xffffffffu, sum, off), up_own = __shfl_up_sync(0xffffffffu, own, off);
+        if (lane >= off) {
+          sum += up;
+          own += up_own;
+        }
       }
-      if (lane == 31) scan[warp] = sum;
+      if (lane == 31) scan[warp] = make_uint2(sum, own);
       all = sum - all;
+      here = own - here;
     }
     __syncthreads();
     if (threadIdx.x < kDigits) {
       uint32_t base = before + all;
-      for (int w = 0; w < warp; ++w) base += scan[w];
-      first_of[threadIdx.x] = base;
+      for (int w = 0; w < warp; ++w) {
+        base += scan[w].x;
+        here += scan[w].y;
+      }
+      first_of[threadIdx.x] = make_uint2(base, here);
     }
     __syncthreads();
-    uint32_t* key_out = s.key[pass & 1];
-    uint32_t* pos_out = s.pos[pass & 1];
-    auto place = [&](bool in, uint32_t key, uint32_t pos, uint32_t same) {
-      const uint32_t digit = (key >> shift) & (kDigits - 1);
+    uint2* pair_out = s.pair[pass & 1];
+    auto place = [&](bool in, uint2 pair, uint32_t same) {
+      const uint32_t digit = (pair.x >> shift) & (kDigits - 1);
       uint32_t slot = 0;
-      if (in) slot = first_of[digit] + hist[warp][digit] + __popc(same & below);
+      if (in) slot = (staged ? first_of[digit].y : first_of[digit].x) + hist[warp][digit] + __popc(same & below);
       __syncwarp();
       if (in && (same & below) == 0) hist[warp][digit] += __popc(same);
       __syncwarp();
-      if (in) {
-        key_out[slot] = key;
-        pos_out[slot] = pos;
-      }
+      if (in) (staged ? local : pair_out)[slot] = pair;
     };
 #pragma unroll
     for (int r = 0; r < kHeld; ++r)
-      if (first + 32 * r < last) place(first + 32 * r + lane < last, held[r], held_pos[r], held_same[r]);
+      if (first + 32 * r < last) place(first + 32 * r + lane < last, held[r], held_same[r]);
     for (int64_t i = first + 32 * kHeld; i < last; i += 32) {
       const bool in = i + lane < last;
-      const uint32_t key = in ? key_of(i + lane) : 0;
-      place(in, key, in ? pos_of(i + lane) : 0, equals(in, key));
+      const uint2 pair = in ? pair_of(i + lane) : make_uint2(0, 0);
+      place(in, pair, equals(in, pair.x));
+    }
+    if (staged) {  // sorted within the CTA first, so that a digit's elements leave side by side
+      __syncthreads();
+      const int64_t start = rank * kSortWarps * span;
+      const int elements = static_cast<int>(max(int64_t{0}, min(n - start, kSortWarps * span)));
+      for (int i = threadIdx.x; i < elements; i += kSortThreads) {
+        const uint2 pair = local[i];
+        const uint2 first_one = first_of[(pair.x >> shift) & (kDigits - 1)];
+        pair_out[first_one.x + static_cast<uint32_t>(i) - first_one.y] = pair;
+      }
     }
     cluster.sync();  // also orders this pass's keys in global memory before the next pass reads them
   }
@@ -257,11 +275,12 @@ __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads
 sort_fill_kernel(const void* tokens, int token_bytes, int64_t n, Sorted s, int passes, Dense out, int bytes_each) {
   __shared__ uint32_t hist[kSortWarps][kDigits];
   __shared__ uint32_t totals[kDigits];
-  __shared__ uint32_t scan[kDigits / 32];
-  __shared__ uint32_t first_of[kDigits];
+  __shared__ uint2 scan[kDigits / 32];
+  __shared__ uint2 first_of[kDigits];  // of the cluster and of the CTA
+  extern __shared__ uint2 local[];     // the CTA's elements, where a warp holds its own
   cg::cluster_group cluster = cg::this_cluster();
   if (blockIdx.x < kSortCtas) {
-    sort_tokens(cluster, tokens, token_bytes, n, out.rows, s, passes, hist, totals, scan, first_of);
+    sort_tokens(cluster, tokens, token_bytes, n, out.rows, s, passes, hist, totals, scan, first_of, local);
     return;
   }
   // Zero is all bits clear in every type.  The CTAs share the 16-byte vectors of contiguous rows, or take
@@ -295,7 +314,7 @@ struct Partials {
 // 32,768 x 2,048 bf16 31.7 us, 4.2 TB/s.
 template <typename In, typename O, bool kAligned>
 __global__ void __launch_bounds__(kSegmentThreads, kAligned ? 8 : 6)
-segment_kernel(const uint32_t* __restrict__ key, const uint32_t* __restrict__ pos, int64_t n,
+segment_kernel(const uint2* __restrict__ sorted, int64_t n,
                int tile, Dense grad, float scale, Dense out, Partials partials, int slices) {
   constexpr int U = kAligned ? 8 : 4;  // rows in flight per thread
   constexpr int V = 16 / static_cast<int>(sizeof(In));
@@ -307,9 +326,10 @@ segment_kernel(const uint32_t* __restrict__ key, const uint32_t* __restrict__ po
   const int count = static_cast<int>(min(n - i0, static_cast<int64_t>(tile)));
   if (threadIdx.x < count + 2) {
     const int64_t i = i0 + threadIdx.x - 1;
-    keys[threadIdx.x] = i >= 0 && i < n ? __ldg(key + i) : ~0u;  // beyond the ends: no token's key
+    const uint2 pair = i >= 0 && i < n ? __ldg(sorted + i) : make_uint2(~0u, 0);  // beyond the ends: no token's key
+    keys[threadIdx.x] = pair.x;
+    if (threadIdx.x >= 1 && threadIdx.x <= count) places[threadIdx.x - 1] = pair.y;
   }
-  if (threadIdx.x < count) places[threadIdx.x] = __ldg(pos + i0 + threadIdx.x);
   __syncthreads();
   if (c >= grad.cols) return;
   const uint32_t limit = static_cast<uint32_t>(out.rows);
@@ -374,19 +394,20 @@ segment_kernel(const uint32_t* __restrict__ key, const uint32_t* __restrict__ po
 // A chain of dependent loads (keys, then partials): 8.9 us for 32,768 x 2,048.
 template <typename O>
 __global__ void __launch_bounds__(32 * kJoinWarps)
-join_kernel(const uint32_t* __restrict__ key, int64_t n, int tile, float scale, Dense out,
+join_kernel(const uint2* __restrict__ sorted, int64_t n, int tile, float scale, Dense out,
             Partials partials) {
   __shared__ float4 sums[kJoinWarps][32];
   const int64_t j = blockIdx.x, i1 = (j + 1) * tile;
   if (i1 >= n) return;
-  const uint32_t run = __ldg(key + i1 - 1), after = __ldg(key + i1), ahead = j > 0 ? __ldg(key + j * tile - 1) : ~0u;
+  auto key = [&](int64_t i) { return __ldg(&sorted[i].x); };
+  const uint32_t run = key(i1 - 1), after = key(i1), ahead = j > 0 ? key(j * tile - 1) : ~0u;
   if (run >= static_cast<uint32_t>(out.rows) || after != run || ahead == run) return;  // ahead: it started earlier
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   // The last tile that the run reaches: 32 tiles' first keys at a time.
   int64_t last = j;
   for (;;) {
     const int64_t first = (last + 1 + lane) * tile;
-    const uint32_t stop = __ballot_sync(0xffffffffu, first >= n || __ldg(key + min(first, n - 1)) != run);
+    const uint32_t stop = __ballot_sync(0xffffffffu, first >= n || key(min(first, n - 1)) != run);
     last += stop ? __ffs(stop) - 1 : 32;
     if (stop) break;
   }
@@ -479,27 +500,29 @@ cudaError_t gradient(const void* tokens, int token_bytes, const Dense& grad, flo
   const int64_t n = grad.rows;
   const int64_t padded = (n + 3) / 4 * 4;
   auto* words = static_cast<uint32_t*>(workspace);
-  const Sorted s{{words, words + padded}, {words + 2 * padded, words + 3 * padded}};
+  const Sorted s{{reinterpret_cast<uint2*>(words), reinterpret_cast<uint2*>(words) + padded}};
   const Partials partials{reinterpret_cast<float*>(words + 4 * padded), partial_pitch(out.cols)};
   int passes = 1;
   while (passes < 4 && (out.rows >> (8 * passes)) > 0) ++passes;
   const int64_t fill = (out.rows * out.cols * static_cast<int64_t>(sizeof(O)) / 16 + kSortThreads - 1) / kSortThreads;
   const int64_t clusters = 1 + std::min<int64_t>((fill + kSortCtas - 1) / kSortCtas + 1, info.sm_count / kSortCtas * 2);
-  sort_fill_kernel<<<static_cast<unsigned>(clusters * kSortCtas), kSortThreads, 0, stream>>>(
+  const int shared = sort_span(n) <= 32 * kHeld ? static_cast<int>(sort_span(n)) * kSortWarps * 8 : 0;
+  static SharedLimit limit;
+  if ((err = limit.raise(sort_fill_kernel, 32 * kHeld * kSortWarps * 8)) != cudaSuccess) return err;
+  sort_fill_kernel<<<static_cast<unsigned>(clusters * kSortCtas), kSortThreads, shared, stream>>>(
       tokens, token_bytes, n, s, n > 0 ? passes : 0, out, static_cast<int>(sizeof(O)));
   if ((err = cudaGetLastError()) != cudaSuccess || n == 0) return err;
-  const uint32_t* key = s.key[(passes - 1) & 1];
-  const uint32_t* pos = s.pos[(passes - 1) & 1];
+  const uint2* sorted = s.pair[(passes - 1) & 1];
   const int64_t slices = (out.cols + V * kSegmentThreads - 1) / (V * kSegmentThreads);
   const int tile = static_cast<int>(tile_of(n, slices));
   const int64_t tiles = (n + tile - 1) / tile;
   if (tiles * slices > 0x7fffffff) return cudaErrorInvalidConfiguration;
   auto* kernel = vectors_fit<In, O>(grad, out) ? segment_kernel<In, O, true> : segment_kernel<In, O, false>;
-  kernel<<<static_cast<unsigned>(tiles * slices), kSegmentThreads, 0, stream>>>(key, pos, n, tile, grad, scale, out, partials,
+  kernel<<<static_cast<unsigned>(tiles * slices), kSegmentThreads, 0, stream>>>(sorted, n, tile, grad, scale, out, partials,
                                                                                 static_cast<int>(slices));
   if ((err = cudaGetLastError()) != cudaSuccess || tiles == 1) return err;
   const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(std::min<int64_t>(16, std::max((out.cols + 1023) / 1024, std::min<int64_t>(4, (out.cols + 255) / 256)))));
-  join_kernel<O><<<grid, 32 * kJoinWarps, 0, stream>>>(key, n, tile, scale, out, partials);
+  join_kernel<O><<<grid, 32 * kJoinWarps, 0, stream>>>(sorted, n, tile, scale, out, partials);
   return cudaGetLastError();
 }
 
