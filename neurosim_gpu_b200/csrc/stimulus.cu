@@ -505,10 +505,15 @@ cudaError_t gradient(const void* tokens, int token_bytes, const Dense& grad, flo
   int passes = 1;
   while (passes < 4 && (out.rows >> (8 * passes)) > 0) ++passes;
   const int64_t fill = (out.rows * out.cols * static_cast<int64_t>(sizeof(O)) / 16 + kSortThreads - 1) / kSortThreads;
-  const int64_t clusters = 1 + std::min<int64_t>((fill + kSortCtas - 1) / kSortCtas + 1, info.sm_count / kSortCtas * 2);
   const int shared = sort_span(n) <= 32 * kHeld ? static_cast<int>(sort_span(n)) * kSortWarps * 8 : 0;
   static SharedLimit limit;
-  if ((err = limit.raise(sort_fill_kernel, 32 * kHeld * kSortWarps * 8)) != cudaSuccess) return err;
+  constexpr int kMost = 32 * kHeld * kSortWarps * 8;
+  if ((err = limit.raise(sort_fill_kernel, kMost)) != cudaSuccess) return err;
+  // As many clusters as run at once, 30 (32,000 x 1,024 f32: 30.5 us; with 34, of which some wait, 35.6).
+  static ClusterLimit at_once;
+  int most = 0;
+  if ((err = at_once.most(sort_fill_kernel, kSortCtas, kSortThreads, kMost, &most)) != cudaSuccess) return err;
+  const int64_t clusters = 1 + std::min<int64_t>((fill + kSortCtas - 1) / kSortCtas + 1, std::max(1, most - 1));
   sort_fill_kernel<<<static_cast<unsigned>(clusters * kSortCtas), kSortThreads, shared, stream>>>(
       tokens, token_bytes, n, s, n > 0 ? passes : 0, out, static_cast<int>(sizeof(O)));
   if ((err = cudaGetLastError()) != cudaSuccess || n == 0) return err;
