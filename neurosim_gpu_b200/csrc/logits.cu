@@ -189,8 +189,8 @@ logits_kernel(LogitsArgs a, int ctas, int room) {
     auto word = [](uint32_t two) { return (two & 1 ? 0xffffu : 0u) | (two & 2 ? 0xffff0000u : 0u); };
     const uint32_t byte = threadIdx.x;
     masks[byte] = make_uint4(word(byte), word(byte >> 2), word(byte >> 4), word(byte >> 6));
-    if (!kHistory) __syncthreads();  // a history has barriers of its own
   }
+  if (kTable && !kHistory) __syncthreads();  // a history has barriers of its own
   const Penalties p{row_value(a.repetition, b), row_value(a.presence, b), row_value(a.frequency, b)};
 
   // Vector i of the row covers tokens [i * P - shift, + P): vectors start on 16-byte boundaries.
@@ -443,7 +443,7 @@ cudaError_t adjust_rows(const LogitsArgs& a, cudaStream_t stream) {
   cudaError_t err = device_info(&info);
   if (err != cudaSuccess) return err;
   // Few CTAs to a row count its history less often; more fill the GPU: three or four of 256 threads per SM,
-  // as long as they have 2,048 tokens each (256 x 131,071 bf16: 60 us with four to a row, 77 with one).
+  // as long as they have 2,048 tokens each (256 x 131,071 bf16: 60 us with two to a row, 77 with one).
   // Where even eight to a row leave SMs idle, they get 1,024 threads (1 x 131,072 f32, 4,096 tokens of
   // history: 13.3 us against 16.0 with 256).
   unsigned ctas = 1, threads = 256;

@@ -225,3 +225,13 @@ def test_long_histories_in_place(dtype, rows, vocabulary, length):
     x = logits.cuda()
     again, same = adjust_logits(x, out=x, choose=True, **device)
     assert again is x and torch.equal(x, got) and torch.equal(same, choice)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocabulary", [(1, 131_072), (3, 40_001), (18, 33_000), (20, 33_000)])
+def test_few_long_rows_without_a_history(dtype, rows, vocabulary):
+    logits = (3 * torch.randn(rows, vocabulary, generator=generator(5))).to(dtype)
+    kw = case(rows, vocabulary, 0)
+    check(logits, dtype)
+    check(logits, dtype, mask=kw["mask"], bias=kw["bias"])
