@@ -11,7 +11,7 @@
 // ascending t, in float32, cut at fixed tiles of the sorted order and joined in
 // ascending tile order.  Three launches:
 //   1. sort_fill_kernel: one cluster sorts (token, t) stably, byte by byte (radix
-//      sort; the keys stay in L2), while all other clusters write the table's zeros.
+//      sort; the pairs stay in L2), while all other clusters write the table's zeros.
 //      The sort is all latency, the zeros are all bandwidth: neither waits.
 //   2. segment_kernel: one CTA per (tile of the sorted order, slice of the columns)
 //      sums runs of equal tokens; a run inside the tile is written to its row, one
@@ -136,8 +136,10 @@ __host__ __device__ inline int64_t sort_span(int64_t n) {
 // Stable least-significant-byte radix sort of the keys min(token, limit) by one cluster.
 // Warp g of the cluster's 256 owns elements [g * span, (g + 1) * span).  Per pass: each warp
 // counts its digits; a scan over (digit, CTA, warp) gives each warp the first slot of each of
-// its digits; the warp walks its elements again in order and places them.  All latency: 32,768 ids, two
-// passes, 22.8 us; two clusters and more would have to meet in global memory between the passes.
+// its digits; the warp walks its elements again in order and places them: in the CTA's shared memory
+// first, from where each digit's elements leave side by side (single words scattered over global memory:
+// 22.2 us, this way 19.0 for 32,768 ids in two passes), or at once where a warp has too many to hold.
+// All latency; more than one cluster would have to meet in global memory between the passes.
 __device__ void sort_tokens(cg::cluster_group& cluster, const void* tokens, int token_bytes,
                             int64_t n, int64_t limit, const Sorted& s, int passes,
                             uint32_t (*hist)[kDigits], uint32_t* totals, uint2* scan, uint2* first_of, uint2* local) {
@@ -391,7 +393,7 @@ segment_kernel(const uint2* __restrict__ sorted, int64_t n,
 
 // Tile j joins the run that starts in it and goes on into later tiles.  A short run: each of the CTA's
 // warps takes 128 columns; a long one: the warps share its tiles, and their sums are added in warp order.
-// A chain of dependent loads (keys, then partials): 8.9 us for 32,768 x 2,048.
+// A chain of dependent loads (keys, then partials): 9.0 us for 32,768 x 2,048.
 template <typename O>
 __global__ void __launch_bounds__(32 * kJoinWarps)
 join_kernel(const uint2* __restrict__ sorted, int64_t n, int tile, float scale, Dense out,
