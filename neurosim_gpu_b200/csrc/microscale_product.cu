@@ -212,16 +212,17 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
         }
         if (elect_one()) {
           uint8_t* to = stages + ring.stage * S::kStageBytes;
+          const int64_t scale_offset = static_cast<int64_t>(k) * kScaleBytes;  // beyond 2^31 from 2^20 K tiles on
           if (n >= ahead) {
             barrier_arrive_expect(full, S::kStageBytes);
             load_box(to, &lane_map, k * kTileBytes, lane_block(lt) * kLanes, full);
-            load_bytes(to + kLaneBytes + S::kColumnBytes, lane_scales + k * kScaleBytes, kScaleBytes, full);
+            load_bytes(to + kLaneBytes + S::kColumnBytes, lane_scales + scale_offset, kScaleBytes, full);
           }
           load_box(to + kLaneBytes, &column_map, k * kTileBytes, ct * kColumns + (kPair ? rank * S::kColumnRows : 0), full);
           to += kLaneBytes + S::kColumnBytes;
 #pragma unroll
           for (int c = 0; c < S::kBlocks; ++c)
-            load_bytes(to + kScaleBytes * (1 + c), column_scales[c] + k * kScaleBytes, kScaleBytes, full);
+            load_bytes(to + kScaleBytes * (1 + c), column_scales[c] + scale_offset, kScaleBytes, full);
         }
         __syncwarp();
       }
@@ -300,6 +301,7 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
     const int part = (warp - 2) / 4 * S::kOutColumns;  // first column
     int t = 0;
     bool ok = true;  // once a wait has given up, the tiles are walked for their barriers alone
+    const long long sum_polls = kBarrierPolls * (1ll + (k1 - k0) / 1024);  // the wait for all of a tile's products
     for (int tile = first; tile < tiles; tile += step, ++t) {
       int lt, ct;
       place(a, tile, &lt, &ct);
@@ -318,7 +320,7 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
       const bool in = row < a.lane.rows;
       const float row_scale = in ? __ldg(a.lane.scale + (a.lane.per_row ? row : 0)) : 0.0f;
       const float row_bias = in && a.lane.bias ? __ldg(a.lane.bias + row) : 0.0f;
-      if (ok && !barrier_wait(&h.sum_full[b], use & 1, aborted)) {
+      if (ok && !barrier_wait(&h.sum_full[b], use & 1, aborted, sum_polls)) {
         if (lane == 0) give_up(a, aborted, 4);
         ok = false;
       }

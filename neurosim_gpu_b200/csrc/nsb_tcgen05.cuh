@@ -77,8 +77,8 @@ __device__ __forceinline__ void cluster_barrier() {
 constexpr int kBarrierPolls = 1 << 22;
 
 // Bounded wait for the phase `parity` of `bar`; gives up at once when another role of the CTA has (`*aborted`).
-__device__ __forceinline__ bool barrier_wait(uint64_t* bar, uint32_t parity, volatile int* aborted) {
-  for (int i = 0; i < kBarrierPolls; ++i) {
+__device__ __forceinline__ bool barrier_wait(uint64_t* bar, uint32_t parity, volatile int* aborted, long long polls = kBarrierPolls) {
+  for (long long i = 0; i < polls; ++i) {
     if (barrier_try(bar, parity)) return true;
     if ((i & 255) == 255 && *aborted) return false;
   }

@@ -311,6 +311,29 @@ def test_product_of_extreme_scales():
 
 
 @pytest.mark.gpu
+def test_product_past_32_bit_scale_offsets():
+    """2^20 K tiles of 256 columns and more: their block scales lie beyond 2^31 bytes."""
+    columns = 2**28 + 1287
+    at = torch.tensor([0, 100, 2**27 + 3, 2**28 - 1, 2**28, 2**28 + 300, 2**28 + 1286])
+    operands = []
+    for rows, level in ((1, [1, 2, -1, 2, 1, 4, 6]), (3, [2, 1, 3, 1, -2, 6, 1])):
+        codes = torch.zeros(rows, (columns + 31) // 32 * 16, dtype=torch.uint8, device="cuda")
+        scales = torch.zeros(1, (columns + 255) // 256 * 4, 512, dtype=torch.uint8, device="cuda")
+        for i, (c, v) in enumerate(zip(at.tolist(), level)):
+            codes[:, c // 2] = int(np.flatnonzero(LEVELS == v)[0]) << (4 * (c % 2))
+            block = c // 16
+            for r in range(rows):
+                scales[0, block // 4, 16 * r + block % 4] = 0x38 + 8 * (i % 2)  # E4M3 1.0 or 2.0
+        operands.append(Nvfp4Matrix(codes, scales, torch.ones(1, device="cuda"), columns))
+    want = sum(x * y * 4 ** (i % 2) for i, (x, y) in enumerate(zip([1, 2, -1, 2, 1, 4, 6], [2, 1, 3, 1, -2, 6, 1])))
+    got = nvfp4_product(*operands)
+    check_product_status()
+    assert got.tolist() == [[want] * 3]
+    del operands, codes, scales
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
 def test_product_on_a_side_stream_and_in_a_graph():
     x, w = torch.randn(70, 700, generator=generator(8)).cuda(), torch.randn(200, 700, generator=generator(9)).cuda()
     packed = quantize_nvfp4(w, per="tensor")
