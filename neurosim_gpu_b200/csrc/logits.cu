@@ -183,8 +183,8 @@ logits_kernel(LogitsArgs a, int ctas, int room) {
   const float* bias = a.bias ? a.bias + b * a.bias_stride : nullptr;
   const int32_t* mask = a.mask ? a.mask + b * a.mask_stride : nullptr;
   const int32_t* history = a.history + b * a.history_stride;
-  const int length = !kHistory ? 0 : static_cast<int>(a.lengths ? max(int64_t{0}, min(a.history_length, static_cast<int64_t>(__ldg(a.lengths + b)))) : a.history_length);
-  const int prompt = a.prompt_lengths ? __ldg(a.prompt_lengths + b) : 0;
+  const uint32_t length = !kHistory ? 0 : static_cast<uint32_t>(a.lengths ? max(int64_t{0}, min(a.history_length, static_cast<int64_t>(__ldg(a.lengths + b)))) : a.history_length);
+  const uint32_t prompt = a.prompt_lengths ? max(0, __ldg(a.prompt_lengths + b)) : 0;
   if (kTable && threadIdx.x < 256) {
     auto word = [](uint32_t two) { return (two & 1 ? 0xffffu : 0u) | (two & 2 ? 0xffff0000u : 0u); };
     const uint32_t byte = threadIdx.x;
@@ -218,8 +218,9 @@ logits_kernel(LogitsArgs a, int ctas, int room) {
     const int v0 = i0 * P - shift;  // the token of bit 0; may be below 0
     // A batch of the history's tokens: where the bit of each lies, bit | owner << 20, or -1 for one that is
     // not in this part.
-    const int step = together ? ctas * threads : threads, h_first = (together ? rank * threads : 0) + threadIdx.x;
-    auto read = [&](int h0, int (&token)[kBatch]) {
+    // Places in the history are unsigned: a walk ends up to a batch beyond a length just below 2^31.
+    const uint32_t step = together ? ctas * threads : threads, h_first = (together ? rank * threads : 0) + threadIdx.x;
+    auto read = [&](uint32_t h0, int (&token)[kBatch]) {
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) token[j] = h0 + j * step < length ? __ldg(history + h0 + j * step) : -1;
     };
@@ -245,7 +246,7 @@ logits_kernel(LogitsArgs a, int ctas, int room) {
       sync();
       int place[kBatch], token[kBatch];
       read(h_first, token);
-      for (int h0 = h_first; h0 < length; h0 += kBatch * step) {
+      for (uint32_t h0 = h_first; h0 < length; h0 += kBatch * step) {
         locate(token, place);
         read(h0 + kBatch * step, token);
 #pragma unroll
@@ -291,7 +292,7 @@ logits_kernel(LogitsArgs a, int ctas, int room) {
       }
       sync();
       read(h_first, token);
-      for (int h0 = h_first; h0 < length; h0 += kBatch * step) {
+      for (uint32_t h0 = h_first; h0 < length; h0 += kBatch * step) {
         locate(token, place);
         read(h0 + kBatch * step, token);
 #pragma unroll

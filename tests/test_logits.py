@@ -235,3 +235,23 @@ def test_few_long_rows_without_a_history(dtype, rows, vocabulary):
     kw = case(rows, vocabulary, 0)
     check(logits, dtype)
     check(logits, dtype, mask=kw["mask"], bias=kw["bias"])
+
+
+@pytest.mark.gpu
+def test_history_just_below_32_bits():
+    """A walk over the history steps past its end: the place there is beyond 2^31."""
+    length, vocabulary = 2**31 - 1, 40_000
+    history = torch.full((1, length), -1, dtype=torch.int32, device="cuda")
+    history[0, -3:] = torch.tensor([7, 39_999, 7])
+    history[0, 5] = 11
+    logits = torch.ones(1, vocabulary, device="cuda")
+    prompts = torch.tensor([2**31 - 3], dtype=torch.int32, device="cuda")  # the last two are generated
+    got = adjust_logits(logits, history=history, prompt_lengths=prompts, repetition=2.0, frequency=0.25, presence=1.0)
+    want = torch.ones(vocabulary)
+    want[[7, 39_999]] = 0.5 - 0.25 - 1.0
+    want[11] = 0.5
+    assert torch.equal(got[0].cpu(), want)
+    negative = adjust_logits(logits, history=history[:, -3:], prompt_lengths=-prompts, frequency=0.25)  # no prompt
+    assert negative[0, 7] == 0.5 and negative[0, 39_999] == 0.75
+    del history
+    torch.cuda.empty_cache()
