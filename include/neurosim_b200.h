@@ -607,7 +607,8 @@ NSB_API int nsb_nvfp4_quantize(const nsb_matrix* value, int32_t transpose, const
 NSB_API int nsb_nvfp4_dequantize(const nsb_nvfp4* value, const nsb_matrix* out, void* stream);
 
 /* out[m, n] = sum over k of a[m, k] b[n, k], plus bias[n] where bias is given (float32).  Sums are
- * float32; the result depends on the operands only (deterministic).  Bounded waits inside the kernel
+ * float32; the result depends on the operands only (deterministic).  Operands of a product (the matrices
+ * of a training step, both ways round) have fewer than 2^31 - 256 rows.  Bounded waits inside the kernel
  * write a code other than 0 to *status (device, may be NULL) where they give up. */
 NSB_API int nsb_nvfp4_product(const nsb_nvfp4* a, const nsb_nvfp4* b, const float* bias,
                               const nsb_matrix* out, int* status, void* stream);

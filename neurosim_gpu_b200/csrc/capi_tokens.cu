@@ -9,6 +9,7 @@
 namespace {
 
 constexpr int64_t kMost = int64_t{1} << 31;  // rows, columns and tokens are below this
+constexpr int64_t kMostProduct = kMost - 256;  // ... a product's rows below this: its tiles are counted in 32 bits
 
 bool fail(const char* message) { return nsb::set_error(NSB_ERR_ARGUMENT, message), false; }
 
@@ -72,6 +73,10 @@ size_t packed_bytes(int64_t rows, int64_t cols) {
 
 bool sizes_ok(int64_t rows, int64_t cols, int64_t outputs) {
   return rows >= 1 && cols >= 1 && outputs >= 1 && rows < kMost && cols < kMost && outputs < kMost;
+}
+
+bool product_ok(int64_t a_rows, int64_t b_rows) {
+  return a_rows < kMostProduct && b_rows < kMostProduct ? true : fail("a product's matrices must have fewer than 2^31 - 256 rows");
 }
 
 }  // namespace
@@ -162,6 +167,7 @@ int nsb_nvfp4_product(const nsb_nvfp4* a, const nsb_nvfp4* b, const float* bias,
   if (x.cols != y.cols) return nsb::set_error(NSB_ERR_ARGUMENT, "the operands must have the same number of columns");
   if (y.rows < 1 || o.rows != x.rows || o.cols != y.rows)
     return nsb::set_error(NSB_ERR_ARGUMENT, "the product must be [a.rows, b.rows], b.rows >= 1");
+  if (!product_ok(x.rows, y.rows)) return NSB_ERR_ARGUMENT;
   if (reinterpret_cast<uintptr_t>(bias) % 4 != 0) return nsb::set_error(NSB_ERR_ARGUMENT, "the bias must be 4-byte aligned");
   nsb::set_error(NSB_OK, "");
   if (x.rows == 0) return NSB_OK;
@@ -183,6 +189,7 @@ int nsb_nvfp4_readout(const nsb_matrix* state, const nsb_nvfp4* weight, const fl
   if (x.cols != w.cols) return nsb::set_error(NSB_ERR_ARGUMENT, "states and weights must have the same number of columns");
   if (w.rows < 1 || o.rows != x.rows || o.cols != w.rows)
     return nsb::set_error(NSB_ERR_ARGUMENT, "the output must be [state.rows, weight.rows], weight.rows >= 1");
+  if (!product_ok(x.rows, w.rows)) return NSB_ERR_ARGUMENT;
   if (reinterpret_cast<uintptr_t>(bias) % 4 != 0) return nsb::set_error(NSB_ERR_ARGUMENT, "the bias must be 4-byte aligned");
   if (!check_workspace(workspace, workspace_bytes, nsb_nvfp4_readout_workspace_size(x.rows, x.cols), 16)) return NSB_ERR_WORKSPACE;
   nsb::set_error(NSB_OK, "");
@@ -213,6 +220,7 @@ int nsb_nvfp4_train_forward(const nsb_matrix* state, const nsb_matrix* weight, c
     return NSB_ERR_ARGUMENT;
   if (x.cols != w.cols || w.rows < 1 || o.rows != x.rows || o.cols != w.rows)
     return nsb::set_error(NSB_ERR_ARGUMENT, "states [M, K], weights [N >= 1, K] and output [M, N] do not fit together");
+  if (!product_ok(x.rows, w.rows)) return NSB_ERR_ARGUMENT;
   if (reinterpret_cast<uintptr_t>(bias) % 4 != 0 || !largest || reinterpret_cast<uintptr_t>(largest) % 4 != 0)
     return nsb::set_error(NSB_ERR_ARGUMENT, "two words for the largest sizes are required; they and the bias must be 4-byte aligned");
   if (!check_workspace(workspace, workspace_bytes, nsb_nvfp4_train_workspace_size(x.rows, x.cols, w.rows), 16)) return NSB_ERR_WORKSPACE;
@@ -241,6 +249,7 @@ int nsb_nvfp4_train_backward(const nsb_matrix* state, const nsb_matrix* weight, 
   if (x.rows < 1 || w.rows < 1 || x.cols != w.cols || d.rows != x.rows || d.cols != w.rows ||
       (state_grad && (dx.rows != x.rows || dx.cols != x.cols)) || (weight_grad && (dw.rows != w.rows || dw.cols != w.cols)))
     return nsb::set_error(NSB_ERR_ARGUMENT, "states [M >= 1, K], weights [N >= 1, K], the output's gradient [M, N] and the gradients do not fit together");
+  if (!product_ok(x.rows, w.rows) || !product_ok(x.cols, x.cols)) return NSB_ERR_ARGUMENT;
   if (!largest || reinterpret_cast<uintptr_t>(largest) % 4 != 0 || reinterpret_cast<uintptr_t>(bias_grad) % 4 != 0)
     return nsb::set_error(NSB_ERR_ARGUMENT, "the largest sizes of the forward call are required; they and the bias's gradient must be 4-byte aligned");
   if (!check_workspace(workspace, workspace_bytes, nsb_nvfp4_train_workspace_size(x.rows, x.cols, w.rows), 16)) return NSB_ERR_WORKSPACE;

@@ -141,6 +141,27 @@ def test_entry_points_refuse_bad_arguments():
     assert lib.nsb_column_sums(ctypes.byref(value), p, p, 1, None) == -3
 
 
+def test_products_refuse_rows_that_32_bit_tiles_cannot_count():
+    lib = native.load_library()
+    p, rows = 0x1000, 2**31 - 256  # never read: the checks fail first
+
+    def packed(rows):
+        return ctypes.byref(native._Nvfp4(rows, 16, p, 16, p, p, 1))
+
+    def dense(rows, cols):
+        return ctypes.byref(native._Matrix(p, rows, cols, cols, 0))
+
+    for m, n in ((rows, 6), (6, rows)):
+        assert lib.nsb_nvfp4_product(packed(m), packed(n), None, dense(m, n), None, None) == -1
+        assert b"2^31 - 256" in lib.nsb_last_error()
+        assert lib.nsb_nvfp4_readout(dense(m, 16), packed(n), None, dense(m, n), p, 2**60, None, None) == -1
+        assert lib.nsb_nvfp4_train_forward(dense(m, 16), dense(n, 16), None, dense(m, n), p, p, 2**60, None, None) == -1
+        assert lib.nsb_nvfp4_train_backward(dense(m, 16), dense(n, 16), dense(m, n), p, dense(m, 16), dense(n, 16), None, p, 2**60,
+                                            None, None) == -1
+    assert lib.nsb_nvfp4_train_backward(dense(2, rows), dense(3, rows), dense(2, 3), p, dense(2, rows), dense(3, rows), None, p, 2**60,
+                                        None, None) == -1
+
+
 def test_functions_refuse_cpu_tensors():
     with pytest.raises(ValueError, match="CUDA"):
         quantize_nvfp4(torch.zeros(2, 32))
