@@ -45,7 +45,7 @@ extern "C" {
 #define NSB_API
 #endif
 
-#define NSB_ABI_VERSION 15
+#define NSB_ABI_VERSION 16
 
 enum nsb_status {
   NSB_OK = 0,
@@ -612,6 +612,10 @@ NSB_API int nsb_nvfp4_dequantize(const nsb_nvfp4* value, const nsb_matrix* out, 
  * write a code other than 0 to *status (device, may be NULL) where they give up. */
 NSB_API int nsb_nvfp4_product(const nsb_nvfp4* a, const nsb_nvfp4* b, const float* bias,
                               const nsb_matrix* out, int* status, void* stream);
+
+/* How often the bounded waits of later products of this process poll before they give up: below 0 the
+ * default.  For tests: with 0 every product gives up, and leaves its output as it was. */
+NSB_API void nsb_nvfp4_product_wait_limit(int32_t polls);
 
 /* States through packed weights: nsb_nvfp4_quantize of the states (a scale per row) into the workspace
  * (16-byte aligned, contents need not be initialised), then nsb_nvfp4_product with the weights.  The

@@ -175,6 +175,8 @@ int nsb_nvfp4_product(const nsb_nvfp4* a, const nsb_nvfp4* b, const float* bias,
               "nsb_nvfp4_product launch");
 }
 
+void nsb_nvfp4_product_wait_limit(int32_t polls) { nsb::set_product_polls(polls); }
+
 size_t nsb_nvfp4_readout_workspace_size(int64_t rows, int64_t cols) {
   return sizes_ok(rows, cols, 1) ? packed_bytes(rows, cols) : 0;
 }

@@ -31,6 +31,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "nsb_nvfp4.cuh"
 #include "nsb_tcgen05.cuh"
@@ -81,6 +82,7 @@ struct ProductArgs {
   int64_t scale_tiles;  // 512-byte tiles per 128 rows
   int32_t k_tiles, split;
   int32_t lane_tiles, column_tiles;  // lane tiles of 128, of pairs 256
+  int polls;  // of a bounded wait
   bool lane_ready;  // the operand along the lanes was complete before the kernel ahead of this one started
   int* status;
 };
@@ -97,6 +99,7 @@ struct Header {
 static_assert(sizeof(Header) <= kHeader, "header");
 
 __device__ int g_product_status;  // where no status word is given
+std::atomic<int> g_polls{kBarrierPolls};
 
 __device__ __forceinline__ void give_up(const ProductArgs& a, volatile int* aborted, int code) {
   *aborted = 1;
@@ -174,9 +177,10 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
   tcgen05_fence_after();
   const uint32_t tmem = h.tmem;
 
+  int loads = 0;  // K tiles that warp 0 has asked for
   if (warp == 0) {  // loads
     Ring<S::kStages> ring;
-    int n = 0, ahead = 0;
+    int ahead = 0;
     bool ok = true;
     if (a.lane_ready && first < tiles) {  // its first stages' share while the kernel ahead still runs
       int lt, ct;
@@ -204,16 +208,16 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
         const int64_t block = static_cast<int64_t>(ct) * S::kBlocks + c;
         column_scales[c] = a.column.block_scales + (block * 128 < a.column.rows ? block : 0) * a.scale_tiles * 512;
       }
-      for (int k = k0; k < k1; ++k, ++n, ring.next()) {
+      for (int k = k0; k < k1; ++k, ++loads, ring.next()) {
         uint64_t* full = &h.full[ring.stage];
-        if (ring.round > 0 && !barrier_wait(&h.empty[ring.stage], (ring.round - 1) & 1, aborted)) {
+        if (ring.round > 0 && !barrier_wait(&h.empty[ring.stage], (ring.round - 1) & 1, aborted, a.polls)) {
           ok = false;
           break;
         }
         if (elect_one()) {
           uint8_t* to = stages + ring.stage * S::kStageBytes;
           const int64_t scale_offset = static_cast<int64_t>(k) * kScaleBytes;  // beyond 2^31 from 2^20 K tiles on
-          if (n >= ahead) {
+          if (loads >= ahead) {
             barrier_arrive_expect(full, S::kStageBytes);
             load_box(to, &lane_map, k * kTileBytes, lane_block(lt) * kLanes, full);
             load_bytes(to + kLaneBytes + S::kColumnBytes, lane_scales + scale_offset, kScaleBytes, full);
@@ -228,16 +232,12 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
       }
     }
     if (!ok && lane == 0) give_up(a, aborted, 1);
-    if (*aborted)  // nothing may land in shared memory after the CTA has gone
-      for (int u = max(0, n - S::kStages); u < n; ++u)
-        for (int i = 0; i < kBarrierPolls && !barrier_try(&h.full[u % S::kStages], (u / S::kStages) & 1); ++i) {
-        }
   } else if (warp == 1 && !issues) {  // the pair's second CTA: its loads are in
     Ring<S::kStages> ring;
     bool ok = true;
     for (int tile = first; ok && tile < tiles; tile += step)
       for (int k = k0; ok && k < k1; ++k, ring.next()) {
-        ok = barrier_wait(&h.full[ring.stage], ring.round & 1, aborted);
+        ok = barrier_wait(&h.full[ring.stage], ring.round & 1, aborted, a.polls);
         if (ok && elect_one()) barrier_arrive_at(&h.peer_full[ring.stage], 0);
         __syncwarp();
       }
@@ -253,7 +253,7 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
       int lt, ct;
       place(a, tile, &lt, &ct);
       const int b = t % S::kSums, use = t / S::kSums;
-      if (use > 0 && !barrier_wait(&h.sum_empty[b], (use - 1) & 1, aborted)) {
+      if (use > 0 && !barrier_wait(&h.sum_empty[b], (use - 1) & 1, aborted, a.polls)) {
         if (lane == 0) give_up(a, aborted, 2);
         break;
       }
@@ -262,8 +262,8 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
       const uint32_t instruction = nvfp4_instruction(kPair ? 2 * kLanes : kLanes, kPair ? kColumns : min(kColumns, (a.column.rows - ct * kColumns + 15) / 16 * 16));
       const uint32_t sum = tmem + b * kColumns;
       for (int k = k0; k < k1; ++k, ring.next()) {
-        if (!barrier_wait(&h.full[ring.stage], ring.round & 1, aborted) ||
-            (kPair && !barrier_wait(&h.peer_full[ring.stage], ring.round & 1, aborted))) {
+        if (!barrier_wait(&h.full[ring.stage], ring.round & 1, aborted, a.polls) ||
+            (kPair && !barrier_wait(&h.peer_full[ring.stage], ring.round & 1, aborted, a.polls))) {
           if (lane == 0) give_up(a, aborted, 3);
           ok = false;
           break;
@@ -290,18 +290,13 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
         __syncwarp();
       }
     }
-    if (*aborted) {
-      if (elect_one()) mma_commit<kPair>(&h.drained);
-      for (int i = 0; i < kBarrierPolls && !barrier_try(&h.drained, 0); ++i) {
-      }
-    }
   } else {  // results: a warp reads lanes 32 (warp % 4) ... of its columns
     grid_wait();  // the scales may be the kernel's ahead, and what it reads may lie where this one writes
     const int quarter = warp & 3, slot = threadIdx.x - 64;
     const int part = (warp - 2) / 4 * S::kOutColumns;  // first column
     int t = 0;
     bool ok = true;  // once a wait has given up, the tiles are walked for their barriers alone
-    const long long sum_polls = kBarrierPolls * (1ll + (k1 - k0) / 1024);  // the wait for all of a tile's products
+    const long long sum_polls = a.polls * (1ll + (k1 - k0) / 1024);  // the wait for all of a tile's products
     for (int tile = first; tile < tiles; tile += step, ++t) {
       int lt, ct;
       place(a, tile, &lt, &ct);
@@ -363,6 +358,15 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
   }
   tcgen05_fence_before();
   __syncthreads();
+  if (*aborted) {  // by any role: no copy may land and no product run after the CTA has gone
+    if (warp == 0)
+      for (int u = max(0, loads - S::kStages); u < loads; ++u) barrier_drain(&h.full[u % S::kStages], (u / S::kStages) & 1);
+    if (warp == 1 && issues) {
+      if (elect_one()) mma_commit<kPair>(&h.drained);
+      barrier_drain(&h.drained, 0);
+    }
+    __syncthreads();
+  }
   if (kPair) {
     cluster_barrier();  // neither CTA goes while the other may still arrive on its barriers or use its memory
   } else if (a.split > 1) {
@@ -489,6 +493,8 @@ cudaError_t launch(const Nvfp4& lane, const Nvfp4& column, ProductArgs a, int sm
 
 }  // namespace
 
+void set_product_polls(int polls) { g_polls.store(polls < 0 ? kBarrierPolls : polls, std::memory_order_relaxed); }
+
 cudaError_t launch_nvfp4_product(const Nvfp4& a, const Nvfp4& b, const float* bias, const Dense& out,
                                  bool b_ready, int* status, cudaStream_t stream) {
   return with_type(out.type, [&](auto zero) {
@@ -500,6 +506,7 @@ cudaError_t launch_nvfp4_product(const Nvfp4& a, const Nvfp4& b, const float* bi
     args.scale_tiles = block_scale_tiles(a.cols);
     args.k_tiles = static_cast<int32_t>((a.cols + 255) / 256);
     args.status = status;
+    args.polls = g_polls.load(std::memory_order_relaxed);
     // Few rows of b (a narrow readout of many states) go along the columns (8,192 x 25 x 4,096: 10.3 us against
     // 20.1 along the lanes; 300 x 25 x 4,096: 6.1 against 10.8); else b along the lanes, where neighbouring
     // lanes write neighbouring outputs.

@@ -76,13 +76,19 @@ __device__ __forceinline__ void cluster_barrier() {
 // Polls before a wait gives up (tens of milliseconds at the least).
 constexpr int kBarrierPolls = 1 << 22;
 
-// Bounded wait for the phase `parity` of `bar`; gives up at once when another role of the CTA has (`*aborted`).
-__device__ __forceinline__ bool barrier_wait(uint64_t* bar, uint32_t parity, volatile int* aborted, long long polls = kBarrierPolls) {
+// Waits for the phase `parity` of `bar`, `polls` times at most; gives up at once when another role of the CTA has (`*aborted`).
+__device__ __forceinline__ bool barrier_wait(uint64_t* bar, uint32_t parity, volatile int* aborted, long long polls) {
   for (long long i = 0; i < polls; ++i) {
     if (barrier_try(bar, parity)) return true;
     if ((i & 255) == 255 && *aborted) return false;
   }
   return false;
+}
+
+// After a wait has given up: for work in flight, which ends by itself; bounded all the same.
+__device__ __forceinline__ void barrier_drain(uint64_t* bar, uint32_t parity) {
+  for (int i = 0; i < kBarrierPolls && !barrier_try(bar, parity); ++i) {
+  }
 }
 
 // ---------------------------------------------------------------------------

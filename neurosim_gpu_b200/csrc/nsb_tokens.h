@@ -79,6 +79,7 @@ cudaError_t launch_column_sums(const Dense& value, float* out, void* workspace, 
 // b_ready: b was complete before the kernel ahead in the stream started.
 cudaError_t launch_nvfp4_product(const Nvfp4& a, const Nvfp4& b, const float* bias, const Dense& out,
                                  bool b_ready, int* status, cudaStream_t stream);
+void set_product_polls(int polls);
 
 // logits.cu
 struct LogitsArgs {

@@ -169,7 +169,8 @@ EXPORTED_SYMBOLS = ("nsb_dendritic_step", "nsb_csr_propagate",
                     "nsb_tiled_propagate_rows_gated", "nsb_stimulus_drive",
                     "nsb_stimulus_gradient_workspace_size", "nsb_stimulus_gradient",
                     "nsb_nvfp4_quantize_workspace_size", "nsb_nvfp4_quantize",
-                    "nsb_nvfp4_dequantize", "nsb_nvfp4_product", "nsb_nvfp4_readout_workspace_size",
+                    "nsb_nvfp4_dequantize", "nsb_nvfp4_product", "nsb_nvfp4_product_wait_limit",
+                    "nsb_nvfp4_readout_workspace_size",
                     "nsb_nvfp4_readout", "nsb_nvfp4_train_workspace_size",
                     "nsb_nvfp4_train_forward", "nsb_nvfp4_train_backward",
                     "nsb_column_sums_workspace_size",
@@ -271,6 +272,7 @@ def load_library() -> ctypes.CDLL:
     lib.nsb_nvfp4_quantize.argtypes = [p(_Matrix), i32, p(_Nvfp4), ptr, i32, ptr, size, ptr]
     lib.nsb_nvfp4_dequantize.argtypes = [p(_Nvfp4), p(_Matrix), ptr]
     lib.nsb_nvfp4_product.argtypes = [p(_Nvfp4), p(_Nvfp4), ptr, p(_Matrix), ptr, ptr]
+    lib.nsb_nvfp4_product_wait_limit.argtypes = [i32]
     lib.nsb_nvfp4_readout_workspace_size.argtypes = [i64, i64]
     lib.nsb_nvfp4_readout_workspace_size.restype = size
     lib.nsb_nvfp4_readout.argtypes = [p(_Matrix), p(_Nvfp4), ptr, p(_Matrix), ptr, size, ptr, ptr]
@@ -288,7 +290,7 @@ def load_library() -> ctypes.CDLL:
     lib.nsb_abi_version.restype = ctypes.c_int
     for name in EXPORTED_SYMBOLS:
         getattr(lib, name).restype = getattr(lib, name).restype or ctypes.c_int
-    if lib.nsb_abi_version() != 15:
+    if lib.nsb_abi_version() != 16:
         raise RuntimeError("libneurosim_b200.so ABI version mismatch")
     return lib
 

@@ -354,6 +354,35 @@ def test_product_past_32_bit_scale_offsets():
     torch.cuda.empty_cache()
 
 
+# One of each tile, split along K or not, and pairs of CTAs with few and with many K tiles.
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 129, 4096), (17, 300, 255), (64, 131, 2570), (130, 2, 320), (256, 256, 2048),
+                                   (2048, 2560, 520), (2300, 2420, 6000), (2304, 20_000, 64)])
+def test_waits_that_run_out_report_and_leave_the_context_usable(m, n, k):
+    lib = native.load_library()
+    a, x = exact_operand(m, k, 1)
+    b, y = exact_operand(n, k, 2)
+    out, status = torch.full((m, n), 7.0, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    view = native.dense_matrix(out, "out")
+
+    def product():
+        native.token_call(out, lib.nsb_nvfp4_product, ctypes.byref(a._view), ctypes.byref(b._view), None, ctypes.byref(view),
+                          status.data_ptr())
+
+    lib.nsb_nvfp4_product_wait_limit(0)  # every wait gives up at once
+    try:
+        for _ in range(3):
+            product()
+        torch.cuda.synchronize()
+    finally:
+        lib.nsb_nvfp4_product_wait_limit(-1)
+    assert int(status) != 0 and bool((out == 7.0).all())
+    status.zero_()
+    product()
+    assert int(status) == 0
+    assert torch.equal(out.cpu().double(), x @ y.t())
+
+
 @pytest.mark.gpu
 def test_product_on_a_side_stream_and_in_a_graph():
     x, w = torch.randn(70, 700, generator=generator(8)).cuda(), torch.randn(200, 700, generator=generator(9)).cuda()
