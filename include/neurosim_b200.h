@@ -609,13 +609,19 @@ NSB_API int nsb_nvfp4_dequantize(const nsb_nvfp4* value, const nsb_matrix* out, 
 /* out[m, n] = sum over k of a[m, k] b[n, k], plus bias[n] where bias is given (float32).  Sums are
  * float32; the result depends on the operands only (deterministic).  Operands of a product (the matrices
  * of a training step, both ways round) have fewer than 2^31 - 256 rows.  Bounded waits inside the kernel
- * write a code other than 0 to *status (device, may be NULL) where they give up. */
+ * write a code other than 0 to *status (device; NULL: a word of the library's, see nsb_nvfp4_product_status)
+ * where they give up; part of `out` is then not written. */
 NSB_API int nsb_nvfp4_product(const nsb_nvfp4* a, const nsb_nvfp4* b, const float* bias,
                               const nsb_matrix* out, int* status, void* stream);
 
 /* How often the bounded waits of later products of this process poll before they give up: below 0 the
  * default.  For tests: with 0 every product gives up, and leaves its output as it was. */
 NSB_API void nsb_nvfp4_product_wait_limit(int32_t polls);
+
+/* *code (host) = the code that products with no status word of their own have left on the current device
+ * (0: none), which is then cleared.  The word is the library's, so products may be captured at any time.
+ * Waits for `stream`: products on other streams count once they are complete. */
+NSB_API int nsb_nvfp4_product_status(int32_t* code, void* stream);
 
 /* States through packed weights: nsb_nvfp4_quantize of the states (a scale per row) into the workspace
  * (16-byte aligned, contents need not be initialised), then nsb_nvfp4_product with the weights.  The

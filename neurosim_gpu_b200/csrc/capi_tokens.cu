@@ -177,6 +177,12 @@ int nsb_nvfp4_product(const nsb_nvfp4* a, const nsb_nvfp4* b, const float* bias,
 
 void nsb_nvfp4_product_wait_limit(int32_t polls) { nsb::set_product_polls(polls); }
 
+int nsb_nvfp4_product_status(int32_t* code, void* stream) {
+  if (!code) return nsb::set_error(NSB_ERR_ARGUMENT, "a place for the code is required");
+  nsb::set_error(NSB_OK, "");
+  return done(nsb::take_product_status(code, static_cast<cudaStream_t>(stream)), "nsb_nvfp4_product_status");
+}
+
 size_t nsb_nvfp4_readout_workspace_size(int64_t rows, int64_t cols) {
   return sizes_ok(rows, cols, 1) ? packed_bytes(rows, cols) : 0;
 }

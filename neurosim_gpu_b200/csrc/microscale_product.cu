@@ -495,6 +495,15 @@ cudaError_t launch(const Nvfp4& lane, const Nvfp4& column, ProductArgs a, int sm
 
 void set_product_polls(int polls) { g_polls.store(polls < 0 ? kBarrierPolls : polls, std::memory_order_relaxed); }
 
+cudaError_t take_product_status(int* code, cudaStream_t stream) {
+  void* word = nullptr;
+  cudaError_t err = cudaGetSymbolAddress(&word, g_product_status);
+  if (err == cudaSuccess) err = cudaMemcpyAsync(code, word, sizeof(int), cudaMemcpyDeviceToHost, stream);
+  if (err == cudaSuccess) err = cudaStreamSynchronize(stream);
+  if (err == cudaSuccess && *code != 0) err = cudaMemsetAsync(word, 0, sizeof(int), stream);
+  return err;
+}
+
 cudaError_t launch_nvfp4_product(const Nvfp4& a, const Nvfp4& b, const float* bias, const Dense& out,
                                  bool b_ready, int* status, cudaStream_t stream) {
   return with_type(out.type, [&](auto zero) {

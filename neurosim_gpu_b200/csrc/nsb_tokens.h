@@ -80,6 +80,7 @@ cudaError_t launch_column_sums(const Dense& value, float* out, void* workspace, 
 cudaError_t launch_nvfp4_product(const Nvfp4& a, const Nvfp4& b, const float* bias, const Dense& out,
                                  bool b_ready, int* status, cudaStream_t stream);
 void set_product_polls(int polls);
+cudaError_t take_product_status(int* code, cudaStream_t stream);
 
 // logits.cu
 struct LogitsArgs {

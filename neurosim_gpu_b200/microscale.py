@@ -16,11 +16,10 @@ A row of the result depends on its own state alone, not on the rest of the batch
 from __future__ import annotations
 
 import ctypes
-import functools
 
 import torch
 
-from .native import VALUE_TYPES, _Matrix, _Nvfp4, dense_matrix, load_library, token_call
+from .native import VALUE_TYPES, _Matrix, _Nvfp4, _raise_on_status, dense_matrix, load_library, token_call
 
 
 class Nvfp4Matrix:
@@ -126,24 +125,17 @@ def _quantize(value: torch.Tensor, per_row: bool, transpose: bool) -> Nvfp4Matri
     return packed
 
 
-@functools.lru_cache(maxsize=None)
-def _status(device: int) -> torch.Tensor:
-    """The word that products on a device write an error code to (never inside a capture)."""
-    with torch.inference_mode(False):
-        return torch.zeros(1, device=torch.device("cuda", device), dtype=torch.int32)
-
-
-@functools.lru_cache(maxsize=None)
-def _status_pointer(device: int) -> int:
-    return _status(device).data_ptr()
-
-
 def check_product_status(device: torch.device | str = "cuda") -> None:
-    """Raise if a product on ``device`` gave up on a bounded wait (reads the device)."""
+    """Raise if a product on ``device`` gave up on a bounded wait since the last call, and left part of
+    its result unwritten.  Waits for the current stream; what a graph replays counts like any other call.
+    """
     index = torch.device(device).index
-    code = int(_status(torch.cuda.current_device() if index is None else index).item())
-    if code:
-        raise RuntimeError(f"NVFP4 product pipeline timeout (code {code})")
+    code = ctypes.c_int32(0)
+    with torch.cuda.device(torch.cuda.current_device() if index is None else index):
+        lib = load_library()
+        _raise_on_status(lib, lib.nsb_nvfp4_product_status(ctypes.byref(code), torch.cuda.current_stream().cuda_stream))
+    if code.value:
+        raise RuntimeError(f"NVFP4 product pipeline timeout (code {code.value})")
 
 
 def nvfp4_product(a: Nvfp4Matrix, b: Nvfp4Matrix, *, bias: torch.Tensor | None = None,
@@ -168,7 +160,7 @@ def nvfp4_product(a: Nvfp4Matrix, b: Nvfp4Matrix, *, bias: torch.Tensor | None =
         raise ValueError("out must be [M, N] of the given dtype on the operands' device")
     result = dense_matrix(out, "out")
     token_call(out, load_library().nsb_nvfp4_product, ctypes.byref(a._view), ctypes.byref(b._view),
-               None if bias is None else bias.data_ptr(), ctypes.byref(result), _status_pointer(device))
+               None if bias is None else bias.data_ptr(), ctypes.byref(result), None)
     return out
 
 
@@ -193,7 +185,7 @@ def _readout(state: torch.Tensor, weight: Nvfp4Matrix, bias: torch.Tensor | None
     workspace = state.new_empty(size, dtype=torch.uint8)
     token_call(state, lib.nsb_nvfp4_readout, ctypes.byref(view), ctypes.byref(weight._view),
                None if bias is None else bias.data_ptr(), ctypes.byref(result), workspace.data_ptr(), size,
-               _status_pointer(device))
+               None)
     return out
 
 
@@ -217,7 +209,7 @@ class _Readout(torch.autograd.Function):
         result = _Matrix(out.data_ptr(), x.rows, w.rows, w.rows, VALUE_TYPES[dtype])
         token_call(out, lib.nsb_nvfp4_train_forward, ctypes.byref(x), ctypes.byref(w),
                    None if bias is None else bias.data_ptr(), ctypes.byref(result), largest.data_ptr(),
-                   workspace.data_ptr(), size, _status_pointer(device))
+                   workspace.data_ptr(), size, None)
         return out
 
     @staticmethod
@@ -244,7 +236,7 @@ class _Readout(torch.autograd.Function):
                    ctypes.byref(_Matrix(dx.data_ptr(), x.rows, x.cols, x.cols, x.type)) if wants_state else None,
                    ctypes.byref(_Matrix(dw.data_ptr(), w.rows, w.cols, w.cols, w.type)) if wants_weight else None,
                    db.data_ptr() if wants_bias else None, workspace.data_ptr(), size,
-                   _status_pointer(state.get_device()))
+                   None)
         return dx, dw, db, None
 
 

@@ -170,6 +170,7 @@ EXPORTED_SYMBOLS = ("nsb_dendritic_step", "nsb_csr_propagate",
                     "nsb_stimulus_gradient_workspace_size", "nsb_stimulus_gradient",
                     "nsb_nvfp4_quantize_workspace_size", "nsb_nvfp4_quantize",
                     "nsb_nvfp4_dequantize", "nsb_nvfp4_product", "nsb_nvfp4_product_wait_limit",
+                    "nsb_nvfp4_product_status", "nsb_nvfp4_readout_workspace_size",
                     "nsb_nvfp4_readout_workspace_size",
                     "nsb_nvfp4_readout", "nsb_nvfp4_train_workspace_size",
                     "nsb_nvfp4_train_forward", "nsb_nvfp4_train_backward",
@@ -273,6 +274,7 @@ def load_library() -> ctypes.CDLL:
     lib.nsb_nvfp4_dequantize.argtypes = [p(_Nvfp4), p(_Matrix), ptr]
     lib.nsb_nvfp4_product.argtypes = [p(_Nvfp4), p(_Nvfp4), ptr, p(_Matrix), ptr, ptr]
     lib.nsb_nvfp4_product_wait_limit.argtypes = [i32]
+    lib.nsb_nvfp4_product_status.argtypes = [p(i32), ptr]
     lib.nsb_nvfp4_readout_workspace_size.argtypes = [i64, i64]
     lib.nsb_nvfp4_readout_workspace_size.restype = size
     lib.nsb_nvfp4_readout.argtypes = [p(_Matrix), p(_Nvfp4), ptr, p(_Matrix), ptr, size, ptr, ptr]

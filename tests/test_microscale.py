@@ -3,6 +3,9 @@
 from __future__ import annotations
 
 import ctypes
+import subprocess
+import sys
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -138,6 +141,7 @@ def test_entry_points_refuse_bad_arguments():
     assert forward(weight=native._Matrix(p, 6, 41, 41, 0)) == -1 and backward(dw=native._Matrix(p, 5, 40, 40, 0)) == -1
     assert lib.nsb_nvfp4_dequantize(ctypes.byref(packed()), ctypes.byref(native._Matrix(p, 4, 41, 41, 0)), None) == -1
     assert lib.nsb_column_sums(ctypes.byref(value), None, p, 10**6, None) == -1
+    assert lib.nsb_nvfp4_product_status(None, None) == -1
     assert lib.nsb_column_sums(ctypes.byref(value), p, p, 1, None) == -3
 
 
@@ -381,6 +385,51 @@ def test_waits_that_run_out_report_and_leave_the_context_usable(m, n, k):
     product()
     assert int(status) == 0
     assert torch.equal(out.cpu().double(), x @ y.t())
+
+
+FIRST_PRODUCT_IN_A_CAPTURE = """
+import torch
+from neurosim_gpu_b200 import check_product_status, native, nvfp4_readout, quantize_nvfp4
+lib = native.load_library()
+x = torch.randn(3, 64, device="cuda")
+w = quantize_nvfp4(torch.randn(5, 64, device="cuda"))
+good, bad = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+with torch.cuda.graph(good):  # the process's first product
+    y = nvfp4_readout(x, w)
+check_product_status()        # nothing has run: nothing has failed
+good.replay()
+check_product_status()
+want = nvfp4_readout(x, w)
+assert torch.equal(y, want)
+lib.nsb_nvfp4_product_wait_limit(0)
+with torch.cuda.graph(bad):
+    z = nvfp4_readout(x, w)
+lib.nsb_nvfp4_product_wait_limit(-1)
+bad.replay()
+good.replay()                 # does not wipe the other's code
+try:
+    check_product_status()
+except RuntimeError as e:
+    assert "timeout" in str(e), e
+else:
+    raise AssertionError("the code was lost")
+check_product_status()        # told once
+bad.replay()
+good.replay()
+assert torch.equal(y, want)
+try:
+    check_product_status("cuda:0")
+except RuntimeError:
+    print("kept")
+"""
+
+
+@pytest.mark.gpu
+def test_status_of_products_in_graphs():
+    result = subprocess.run([sys.executable, "-c", FIRST_PRODUCT_IN_A_CAPTURE], capture_output=True, text=True, timeout=300,
+                            cwd=Path(__file__).resolve().parent.parent)
+    assert result.returncode == 0, result.stderr[-2000:]
+    assert result.stdout.strip().endswith("kept")
 
 
 @pytest.mark.gpu
