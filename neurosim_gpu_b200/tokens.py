@@ -39,7 +39,7 @@ def generate_tokens(runtime, table: torch.Tensor, readout: Nvfp4Matrix | torch.T
     if steps < 0 or ticks < 1:
         raise ValueError("steps must not be negative, and ticks be at least 1")
     length = prompt.shape[1]
-    with torch.inference_mode():
+    with torch.no_grad():  # not inference mode: the runtime keeps the states, and may be trained through later
         history = torch.full((batch, length + steps), -1, device=prompt.device, dtype=torch.int32)
         history[:, :length] = prompt.clamp(-1, 2**31 - 1)  # what no table has stays outside it
         prompts = torch.full((batch,), length, device=prompt.device, dtype=torch.int32)
@@ -57,4 +57,4 @@ def generate_tokens(runtime, table: torch.Tensor, readout: Nvfp4Matrix | torch.T
                                       bias=logit_bias, mask=mask, out=logits, choose=True)
             answer[:, new] = choice
             history[:, at + 1] = choice
-    return answer.clone()
+    return answer

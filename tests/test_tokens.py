@@ -106,3 +106,19 @@ def test_training_through_the_network():
             with torch.no_grad():
                 leaf -= 0.2 * grad
     assert float(now) < 0.5 * float(first)
+
+
+@pytest.mark.parametrize("kind", [NativeDendriticMatrixRuntime, NativeDendriticPELSRuntime])
+@pytest.mark.parametrize("batch", [1, 3])
+def test_training_through_a_runtime_that_has_generated(kind, batch):
+    graph, model, state, table, weight, bias, prompt, _ = parts(batch=batch)
+    runtime = kind(graph, model, state, **({} if kind is NativeDendriticMatrixRuntime else {"theta": 0.01}))
+    answer = generate_tokens(runtime, table, weight, prompt, 2)
+    for value in (answer, runtime.state, runtime.dendritic_state, runtime.adaptation_state):
+        assert not value.is_inference() and not value.requires_grad
+    leaves = [t.clone().requires_grad_() for t in (table, weight, bias)]
+    nvfp4_readout(runtime.state, *leaves[1:]).sum().backward()  # keeps the state for its backward pass
+    assert bool(leaves[1].grad.any()) and bool(leaves[2].grad.any())
+    runtime.step(stimulus_drive(answer[:, -1], leaves[0], scale=0.7))
+    (grad,) = torch.autograd.grad(nvfp4_readout(runtime.state, weight, bias).sum(), leaves[0])
+    assert bool(grad[answer[:, -1]].any())
