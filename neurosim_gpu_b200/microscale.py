@@ -10,6 +10,9 @@ laid out row by row for the tensor cores:
 * ``nvfp4_readout`` quantises states row by row and multiplies them with the readout weights:
   packed ones for inference, floating-point ones for training.
 
+A wait inside a product that runs out is reported by ``check_product_status``, which a program calls
+where it reads results back anyway (``generate_tokens`` does).
+
 A row of the result depends on its own state alone, not on the rest of the batch.
 """
 

@@ -9,7 +9,7 @@ from __future__ import annotations
 import torch
 
 from .logits import adjust_logits
-from .microscale import Nvfp4Matrix, nvfp4_readout
+from .microscale import Nvfp4Matrix, check_product_status, nvfp4_readout
 from .stimulus import stimulus_drive
 
 
@@ -27,7 +27,8 @@ def generate_tokens(runtime, table: torch.Tensor, readout: Nvfp4Matrix | torch.T
     (``table`` [V, N]; -1: no stimulus); the states are read out with ``readout`` ([V_out, N], packed
     or floating-point) and ``bias``, and the largest logit after penalties, ``logit_bias`` and
     ``mask`` (see :func:`adjust_logits`) is the next token, -1 where the mask leaves none.  The
-    ``runtime`` (matrix or PELS) is advanced in place.
+    ``runtime`` (matrix or PELS) is advanced in place.  The call ends with the tokens on the device,
+    and with a check that no product gave up (``RuntimeError``, see :func:`check_product_status`).
     """
     batch, neurons = runtime.state.shape
     if prompt.dim() != 2 or prompt.shape[0] != batch or prompt.shape[1] < 1:
@@ -57,4 +58,6 @@ def generate_tokens(runtime, table: torch.Tensor, readout: Nvfp4Matrix | torch.T
                                       bias=logit_bias, mask=mask, out=logits, choose=True)
             answer[:, new] = choice
             history[:, at + 1] = choice
+        if steps:
+            check_product_status(runtime.state.device)
     return answer

@@ -7,7 +7,7 @@ import torch
 
 from _util import make
 from neurosim_gpu_b200 import (NativeDendriticMatrixRuntime, NativeDendriticPELSRuntime, generate_tokens,
-                               nvfp4_readout, quantize_nvfp4, stimulus_drive)
+                               native, nvfp4_readout, quantize_nvfp4, stimulus_drive)
 
 pytestmark = pytest.mark.gpu
 
@@ -122,3 +122,17 @@ def test_training_through_a_runtime_that_has_generated(kind, batch):
     runtime.step(stimulus_drive(answer[:, -1], leaves[0], scale=0.7))
     (grad,) = torch.autograd.grad(nvfp4_readout(runtime.state, weight, bias).sum(), leaves[0])
     assert bool(grad[answer[:, -1]].any())
+
+
+def test_generate_reports_a_product_that_gave_up():
+    graph, model, state, table, weight, bias, prompt, _ = parts()
+    lib = native.load_library()
+    want = generate_tokens(NativeDendriticMatrixRuntime(graph, model, state.clone()), table, weight, prompt, 3, bias=bias)
+    lib.nsb_nvfp4_product_wait_limit(0)
+    try:
+        with pytest.raises(RuntimeError, match="timeout"):
+            generate_tokens(NativeDendriticMatrixRuntime(graph, model, state.clone()), table, weight, prompt, 3, bias=bias)
+    finally:
+        lib.nsb_nvfp4_product_wait_limit(-1)
+    again = generate_tokens(NativeDendriticMatrixRuntime(graph, model, state.clone()), table, weight, prompt, 3, bias=bias)
+    assert torch.equal(again, want)
