@@ -10,7 +10,7 @@ import ctypes
 
 import torch
 
-from .native import _Logits, _Matrix, _RowValues, dense_matrix, load_library, token_call
+from .native import _Logits, _Matrix, _RowValues, dense_matrix, load_library, refuse_gradients, token_call
 
 
 _NONE = (None, 0)
@@ -65,7 +65,11 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
     [V] or [B, V]; ``mask``: int32 [ceil(V / 32)] or [B, ceil(V / 32)], bit v % 32 of word v // 32
     set where token v is allowed.  ``out`` may be ``logits``.  The choice is the lowest index of a
     row's largest adjusted logit, -1 where nothing is above -inf; a NaN is never chosen.
+
+    There is no backward pass: where gradients are recorded, an argument that requires one is refused.
     """
+    refuse_gradients("adjust_logits takes no gradients: call it under torch.no_grad() or on detached tensors",
+                     logits, out, bias, repetition, presence, frequency)
     view = dense_matrix(logits, "logits")
     rows, vocabulary = view.rows, view.cols
     device = logits.device

@@ -348,6 +348,14 @@ def dense_matrix(value: torch.Tensor, name: str) -> _Matrix:
     return _Matrix(value.data_ptr(), rows, cols, row_stride if row_stride > cols else cols, kind)
 
 
+def refuse_gradients(message: str, *values) -> None:
+    """Raise where one of the values requires a gradient, which the call would drop."""
+    if torch.is_grad_enabled():
+        for value in values:
+            if isinstance(value, torch.Tensor) and value.requires_grad:
+                raise ValueError(message)
+
+
 # The current stream as a pointer and the current device: what torch.cuda.current_stream() and
 # current_device() return, without building a Stream object for every call.
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None

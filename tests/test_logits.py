@@ -127,6 +127,33 @@ def test_function_refuses_cpu_tensors():
         adjust_logits(torch.zeros(2, 8))
 
 
+def test_function_refuses_to_drop_a_gradient():
+    x, leaf, row = torch.zeros(2, 8), torch.zeros(2, 8, requires_grad=True), torch.zeros(2, requires_grad=True)
+    for call in (lambda: adjust_logits(leaf), lambda: adjust_logits(x, out=leaf), lambda: adjust_logits(x, bias=leaf),
+                 lambda: adjust_logits(2 * leaf), lambda: adjust_logits(x, repetition=row), lambda: adjust_logits(x, presence=row),
+                 lambda: adjust_logits(x, frequency=row)):
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
+            call()
+
+
+@pytest.mark.gpu
+def test_logits_that_require_a_gradient():
+    """Of a training readout's result: refused, in place and not, and taken under no_grad."""
+    leaf = torch.randn(3, 50, device="cuda", requires_grad=True)
+    y = 2 * leaf
+    before = y.detach().clone()
+    for kw in ({}, {"out": y}, {"choose": True}):
+        with pytest.raises(ValueError, match="gradient"):
+            adjust_logits(y, bias=torch.ones(50, device="cuda"), **kw)
+    assert torch.equal(y, before)
+    with torch.no_grad():
+        got = adjust_logits(y, bias=torch.ones(50, device="cuda"))
+    assert not got.requires_grad and torch.equal(got, before + 1)
+    assert torch.equal(adjust_logits(y.detach(), bias=torch.ones(50, device="cuda")), got)
+
+
 @pytest.mark.gpu
 def test_function_refuses_bad_arguments():
     x = torch.zeros(2, 40, device="cuda")
