@@ -10,7 +10,7 @@ import ctypes
 
 import torch
 
-from .native import _Logits, _Matrix, _RowValues, dense_matrix, load_library, refuse_gradients, token_call
+from .native import _Logits, _Matrix, _RowValues, dense_matrix, load_library, refuse_gradients, token_call, written
 
 
 _NONE = (None, 0)
@@ -73,6 +73,7 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
     view = dense_matrix(logits, "logits")
     rows, vocabulary = view.rows, view.cols
     device = logits.device
+    given = out
     if out is None:
         out = logits.new_empty((rows, vocabulary))
         result = _Matrix(out.data_ptr(), rows, vocabulary, vocabulary, view.type)
@@ -102,4 +103,6 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
         *(_NONE if mask is None else _broadcast(mask, "mask", torch.int32, rows, (vocabulary + 31) // 32, device)),
         choice.data_ptr() if choose else None)
     token_call(logits, load_library().nsb_adjust_logits, ctypes.byref(args))
+    if given is not None:
+        written(out)
     return (out, choice) if choose else out

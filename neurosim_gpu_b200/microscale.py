@@ -22,7 +22,8 @@ import ctypes
 
 import torch
 
-from .native import VALUE_TYPES, _Matrix, _Nvfp4, _raise_on_status, dense_matrix, load_library, token_call
+from .native import (VALUE_TYPES, _Matrix, _Nvfp4, _raise_on_status, dense_matrix, load_library,
+                     token_call, written)
 
 
 class Nvfp4Matrix:
@@ -155,6 +156,7 @@ def nvfp4_product(a: Nvfp4Matrix, b: Nvfp4Matrix, *, bias: torch.Tensor | None =
     if n < 1:
         raise ValueError("the second operand needs at least one row")
     _check_bias(bias, n, device)
+    given = out
     if out is None:
         if dtype not in VALUE_TYPES:
             raise ValueError("dtype must be float32, float16 or bfloat16")
@@ -164,6 +166,8 @@ def nvfp4_product(a: Nvfp4Matrix, b: Nvfp4Matrix, *, bias: torch.Tensor | None =
     result = dense_matrix(out, "out")
     token_call(out, load_library().nsb_nvfp4_product, ctypes.byref(a._view), ctypes.byref(b._view),
                None if bias is None else bias.data_ptr(), ctypes.byref(result), None)
+    if given is not None:
+        written(out)
     return out
 
 

@@ -356,6 +356,12 @@ def refuse_gradients(message: str, *values) -> None:
                 raise ValueError(message)
 
 
+def written(out: torch.Tensor) -> None:
+    """Tell autograd that a call has written a caller's tensor: a backward pass that kept its old values
+    then refuses to use them, as after torch's own in-place operations."""
+    torch.autograd.graph.increment_version(out)
+
+
 # The current stream as a pointer and the current device: what torch.cuda.current_stream() and
 # current_device() return, without building a Stream object for every call.
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None

@@ -14,7 +14,7 @@ import ctypes
 
 import torch
 
-from .native import VALUE_TYPES, _Matrix, dense_matrix, load_library, token_call
+from .native import VALUE_TYPES, _Matrix, dense_matrix, load_library, token_call, written
 
 
 def _tokens(tokens: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
@@ -30,6 +30,7 @@ def _drive(tokens: torch.Tensor, table: torch.Tensor, scale: float, dtype: torch
     view = dense_matrix(table, "table")
     tokens = _tokens(tokens, table)
     shape = (*tokens.shape, view.cols)
+    given = out
     if out is None:
         out = table.new_empty(shape, dtype=dtype)
     elif out.shape != shape or out.dtype != dtype or out.device != table.device:
@@ -39,6 +40,8 @@ def _drive(tokens: torch.Tensor, table: torch.Tensor, scale: float, dtype: torch
     rows = _Matrix(out.data_ptr(), tokens.numel(), view.cols, view.cols, VALUE_TYPES[dtype])
     token_call(table, load_library().nsb_stimulus_drive, tokens.data_ptr(),
                tokens.element_size(), ctypes.byref(view), scale, ctypes.byref(rows))
+    if given is not None:
+        written(out)
     return out
 
 

@@ -6,8 +6,8 @@ import pytest
 import torch
 
 from _util import make
-from neurosim_gpu_b200 import (NativeDendriticMatrixRuntime, NativeDendriticPELSRuntime, generate_tokens,
-                               native, nvfp4_readout, quantize_nvfp4, stimulus_drive)
+from neurosim_gpu_b200 import (NativeDendriticMatrixRuntime, NativeDendriticPELSRuntime, adjust_logits,
+                               generate_tokens, native, nvfp4_product, nvfp4_readout, quantize_nvfp4, stimulus_drive)
 
 pytestmark = pytest.mark.gpu
 
@@ -136,3 +136,20 @@ def test_generate_reports_a_product_that_gave_up():
         lib.nsb_nvfp4_product_wait_limit(-1)
     again = generate_tokens(NativeDendriticMatrixRuntime(graph, model, state.clone()), table, weight, prompt, 3, bias=bias)
     assert torch.equal(again, want)
+
+
+def test_autograd_learns_of_results_written_over_its_tensors():
+    """exp() keeps its result for its backward pass, which refuses once that has been written over."""
+    leaf = torch.randn(4, 40, device="cuda", requires_grad=True)
+    packed = quantize_nvfp4(torch.randn(4, 64, device="cuda")), quantize_nvfp4(torch.randn(40, 64, device="cuda"))
+    tokens = torch.zeros(4, dtype=torch.int64, device="cuda")
+    for write in (lambda y: adjust_logits(y, out=y), lambda y: stimulus_drive(tokens, leaf, out=y),
+                  lambda y: nvfp4_product(*packed, out=y)):
+        y = leaf.exp()
+        with torch.no_grad():
+            assert write(y) is y
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+    with torch.inference_mode():  # its tensors have no version
+        y = torch.zeros(4, 40, device="cuda")
+        assert adjust_logits(y, out=y) is y
