@@ -23,7 +23,7 @@ import ctypes
 import torch
 
 from .native import (VALUE_TYPES, _Matrix, _Nvfp4, _raise_on_status, dense_matrix, load_library,
-                     token_call, written)
+                     refuse_gradients, refuse_tangents, token_call, written)
 
 
 class Nvfp4Matrix:
@@ -87,6 +87,7 @@ class Nvfp4Matrix:
         """The values the codes stand for: level * (block scale * scale), rounded to ``dtype``."""
         if dtype not in VALUE_TYPES:
             raise ValueError("dtype must be float32, float16 or bfloat16")
+        refuse_gradients("dequantize takes no gradients: its scale requires one", self.scale)
         rows, columns = self.shape
         out = self.scale.new_empty((rows, columns), dtype=dtype)
         result = _Matrix(out.data_ptr(), rows, columns, columns, VALUE_TYPES[dtype])
@@ -99,7 +100,8 @@ def quantize_nvfp4(value: torch.Tensor, *, per: str = "row", transpose: bool = F
     """Pack a [M, K] float32, float16 or bfloat16 matrix, or (``transpose``) its transpose.
 
     ``per="row"``: a float32 scale for each row of the result, so that rows do not depend on one
-    another; ``per="tensor"``: one for all.  A row (or tensor) with an infinity or a NaN is packed
+    another; ``per="tensor"``: one for all.  Packing has no derivative: the result takes no part in
+    autograd, whatever ``value`` requires.  A row (or tensor) with an infinity or a NaN is packed
     with the scale NaN, and reads back as NaN everywhere.
     """
     if per not in ("row", "tensor"):
@@ -149,7 +151,9 @@ def nvfp4_product(a: Nvfp4Matrix, b: Nvfp4Matrix, *, bias: torch.Tensor | None =
 
     ``bias``: float32 [N].  The result is rounded once to ``dtype`` and depends on the operands
     alone (the same call gives the same bits).  ``out`` receives it where given (contiguous rows).
+    Nothing here takes a gradient (:func:`nvfp4_readout` does).
     """
+    refuse_gradients("nvfp4_product takes no gradients: use nvfp4_readout, or detached tensors", bias, out, a.scale, b.scale)
     m, n, device = a.rows, b.rows, a.scale.get_device()
     if a.columns != b.columns or device != b.scale.get_device():
         raise ValueError("the operands must have the same number of columns and the same device")
@@ -262,6 +266,8 @@ def nvfp4_readout(state: torch.Tensor, weight: Nvfp4Matrix | torch.Tensor,
     if dtype not in VALUE_TYPES:
         raise ValueError("dtype must be float32, float16 or bfloat16")
     packed = isinstance(weight, Nvfp4Matrix)
+    scale = weight.scale if packed else None
+    refuse_tangents("nvfp4_readout has no forward-mode derivative", state, scale if packed else weight, bias)
     shape = state.shape
     if not shape or shape[-1] != (weight.columns if packed else weight.shape[-1]):
         raise ValueError("states must be [..., K] for weights [N_out, K]")
@@ -270,7 +276,8 @@ def nvfp4_readout(state: torch.Tensor, weight: Nvfp4Matrix | torch.Tensor,
     if (stride != 1 and shape[-1] > 1) or (row_stride < shape[-1] and flat.shape[0] > 1):
         flat = flat.contiguous()  # e.g. the neuron-major states of a batch
     wants = torch.is_grad_enabled() and (state.requires_grad
-                                         or (bias is not None and bias.requires_grad))
+                                         or (bias is not None and bias.requires_grad)
+                                         or (packed and scale.requires_grad))
     if packed:
         if wants:
             raise ValueError("packed weights take no gradients: pass floating-point weights")

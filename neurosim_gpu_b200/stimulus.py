@@ -14,7 +14,8 @@ import ctypes
 
 import torch
 
-from .native import VALUE_TYPES, _Matrix, dense_matrix, load_library, token_call, written
+from .native import (VALUE_TYPES, _Matrix, dense_matrix, load_library, refuse_gradients, refuse_tangents,
+                     token_call, written)
 
 
 def _tokens(tokens: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
@@ -68,14 +69,15 @@ def stimulus_drive(tokens: torch.Tensor, table: torch.Tensor, *, scale: float = 
     ``tokens``: int32 or int64, any shape.  ``table``: [V, N] float32, float16 or bfloat16 with
     contiguous rows.  ``dtype``: the table's (the default) or float32; the product is taken in
     float32 and rounded once.  ``out`` (contiguous) receives the result where given; it cannot be
-    combined with a table that requires a gradient.
+    combined with a table that requires a gradient.  There is no forward-mode derivative.
     """
     dtype = table.dtype if dtype is None else dtype
     if dtype != table.dtype and dtype != torch.float32:
         raise ValueError("dtype must be the table's or float32")
-    if table.requires_grad and torch.is_grad_enabled():
-        if out is not None:
-            raise ValueError("out cannot be given where the table requires a gradient")
+    refuse_tangents("stimulus_drive has no forward-mode derivative", table, out)
+    if out is not None:
+        refuse_gradients("out cannot be given where it or the table requires a gradient", table, out)
+    elif table.requires_grad and torch.is_grad_enabled():
         return _StimulusDrive.apply(tokens, table, scale, dtype)
     return _drive(tokens, table, scale, dtype, out)
 
@@ -86,8 +88,10 @@ def stimulus_gradient(tokens: torch.Tensor, grad: torch.Tensor, rows: int, *, sc
 
     Row v is ``scale`` times the float32 sum of the gradients of its tokens, in an order that the
     tokens alone fix: the same call gives the same bits.  ``dtype``: ``grad``'s (the default), or
-    another where one of the two is float32.
+    another where one of the two is float32.  It is not differentiable itself: a ``grad`` that requires
+    a gradient is refused.
     """
+    refuse_gradients("stimulus_gradient takes no gradients: call it under torch.no_grad() or on a detached grad", grad)
     if grad.dtype not in VALUE_TYPES or not grad.is_cuda:
         raise ValueError("grad must be a CUDA tensor of float32, float16 or bfloat16")
     dtype = grad.dtype if dtype is None else dtype
