@@ -27,7 +27,7 @@
 //
 // Where there are too few tiles for the GPU, a cluster of 2, 4 or 8 CTAs shares a tile along K: each
 // leaves its float32 partial sums in its shared memory, and each adds a part of the columns of all
-// of them in a fixed order (deterministic) over distributed shared memory.
+// of them over distributed shared memory, every column in the same order.
 #include <cuda.h>
 
 #include <algorithm>
@@ -408,10 +408,17 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
           O* to = static_cast<O*>(a.out) + row * a.lane.stride + (column0 + c) * a.column.stride;
 #pragma unroll
           for (int i = 0; i < L; ++i) {
-            float sum = part[u][0].v[i];
+            // Opposite CTAs first: whichever rank a column falls to, the same pairs and the same sums of pairs,
+            // so that equal rows of the operands give equal results.
+            if (a.split == 8) {
 #pragma unroll
-            for (int r = 1; r < 8; ++r)
-              if (r < a.split) sum += part[u][r].v[i];
+              for (int r = 0; r < 4; ++r) part[u][r].v[i] += part[u][r + 4].v[i];
+            }
+            if (a.split >= 4) {
+#pragma unroll
+              for (int r = 0; r < 2; ++r) part[u][r].v[i] += part[u][r + 2].v[i];
+            }
+            const float sum = part[u][0].v[i] + part[u][1].v[i];
             if (i < rows)
               to[i * a.lane.stride] = Values<O>::down(scaled(sum, row_scale[i], scale, a.column.bias ? __ldg(a.column.bias + column0 + c) : row_bias[i]));
           }

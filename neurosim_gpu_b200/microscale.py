@@ -13,7 +13,9 @@ laid out row by row for the tensor cores:
 A wait inside a product that runs out is reported by ``check_product_status``, which a program calls
 where it reads results back anyway (``generate_tokens`` does).
 
-A row of the result depends on its own state alone, not on the rest of the batch.
+A row of states is quantised by itself, whatever else is in the batch, and equal rows of a batch give equal
+results.  The size of the batch decides how a product is cut into tiles and in which order its sums and
+scales are taken: the same row gives results a few float32 roundings apart in batches of different sizes.
 """
 
 from __future__ import annotations

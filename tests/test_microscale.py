@@ -313,6 +313,23 @@ def test_product(dtype, m, n, k):
     check_product_status()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(8, 1001, 5000), (7, 300, 2100), (60, 200, 1100), (512, 130, 4096), (130, 2, 3200), (300, 700, 1300),
+                                   (2304, 600, 1000)])
+def test_equal_rows_give_equal_results(m, n, k):
+    """Wherever in the batch they lie: tiles split along K over 2, 4 and 8 CTAs, whole ones, and pairs."""
+    def wide(rows, seed):  # blocks of many sizes: sums that float32 rounds
+        size = torch.exp(2 * torch.randn(rows, (k + 15) // 16, generator=generator(seed + 1)))
+        return torch.randn(rows, k, generator=generator(seed)) * torch.repeat_interleave(size, 16, 1)[:, :k]
+
+    x = wide(1, 15).cuda().expand(m, -1).contiguous()
+    w = wide(n, 17)
+    w[1::2] = w[0]
+    y = nvfp4_readout(x, quantize_nvfp4(w.cuda(), per="tensor"))
+    assert torch.equal(y, y[:1].expand(m, -1))
+    assert torch.equal(y[:, 1::2], y[:, :1].expand(-1, n // 2))
+
+
 def decode(packed):
     """The float64 values of a packed matrix, from its bytes."""
     codes = packed.codes.cpu().numpy()
