@@ -35,10 +35,11 @@ class Nvfp4Matrix:
     nibble.  ``block_scales``: uint8 E4M3 [ceil(R / 128), 4 * ceil(K / 256), 512]; tile (i, j) holds
     rows 128 i ... and blocks of 16 columns 4 j ..., the scale of row r and block b at byte
     16 (r % 32) + 4 (r % 128 // 32) + b % 4.  ``scale``: float32 [R] or [1].  Codes and block scales
-    beyond K are zero.  The tensors are used as they are, not copied.
+    beyond K are zero.  The tensors are used as they are, not copied, and stay the matrix's for good:
+    kernels read them by their addresses.  It can be copied and pickled.
     """
 
-    __slots__ = ("codes", "block_scales", "scale", "columns", "_view")
+    __slots__ = ("_codes", "_block_scales", "_scale", "_columns", "_view")
 
     def __init__(self, codes: torch.Tensor, block_scales: torch.Tensor, scale: torch.Tensor,
                  columns: int) -> None:
@@ -59,7 +60,7 @@ class Nvfp4Matrix:
             raise ValueError("codes, block_scales and scale must be on one CUDA device")
         if not (codes.is_contiguous() and block_scales.is_contiguous() and scale.is_contiguous()):
             raise ValueError("codes, block_scales and scale must be contiguous")
-        self.codes, self.block_scales, self.scale, self.columns = codes, block_scales, scale, columns
+        self._codes, self._block_scales, self._scale, self._columns = codes, block_scales, scale, columns
         self._view = _Nvfp4(rows, columns, codes.data_ptr(), shape[1], block_scales.data_ptr(),
                             scale.data_ptr(), count)
 
@@ -68,22 +69,41 @@ class Nvfp4Matrix:
              columns: int, count: int) -> "Nvfp4Matrix":
         """Of tensors made for it: nothing to check."""
         self = cls.__new__(cls)
-        self.codes, self.block_scales, self.scale, self.columns = codes, block_scales, scale, columns
+        self._codes, self._block_scales, self._scale, self._columns = codes, block_scales, scale, columns
         self._view = _Nvfp4(rows, columns, codes.data_ptr(), (columns + 31) // 32 * 16,
                             block_scales.data_ptr(), scale.data_ptr(), count)
         return self
 
+    def __reduce__(self):
+        return Nvfp4Matrix, (self._codes, self._block_scales, self._scale, self._columns)
+
+    @property
+    def codes(self) -> torch.Tensor:
+        return self._codes
+
+    @property
+    def block_scales(self) -> torch.Tensor:
+        return self._block_scales
+
+    @property
+    def scale(self) -> torch.Tensor:
+        return self._scale
+
+    @property
+    def columns(self) -> int:
+        return self._columns
+
     @property
     def rows(self) -> int:
-        return self.codes.shape[0]
+        return self._codes.shape[0]
 
     @property
     def shape(self) -> tuple[int, int]:
-        return self.codes.shape[0], self.columns
+        return self._codes.shape[0], self._columns
 
     @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return self._codes.device
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The values the codes stand for: level * (block scale * scale), rounded to ``dtype``."""

@@ -2,7 +2,9 @@
 
 from __future__ import annotations
 
+import copy
 import ctypes
+import pickle
 import subprocess
 import sys
 from pathlib import Path
@@ -224,6 +226,25 @@ def test_quantize_strides_ties_and_small_values():
     zeros = torch.zeros(2, 40)
     zeros[0, 3] = -0.0
     check_packed(quantize_nvfp4(zeros.cuda()), zeros, "row")
+
+
+@pytest.mark.gpu
+def test_packed_matrices_keep_their_tensors_and_can_be_copied():
+    """The kernels go by the tensors' addresses, which an assignment would leave behind."""
+    x = torch.randn(5, 70, generator=generator(18)).cuda()
+    packed = quantize_nvfp4(x)
+    for name in ("codes", "block_scales", "scale", "columns"):
+        with pytest.raises(AttributeError):
+            setattr(packed, name, getattr(packed, name))
+    want = packed.dequantize()
+    copies = [copy.deepcopy(packed), pickle.loads(pickle.dumps(packed)), copy.copy(packed)]
+    assert copies[2].codes.data_ptr() == packed.codes.data_ptr()
+    for other in copies[:2]:
+        assert other.shape == packed.shape and other.codes.data_ptr() != packed.codes.data_ptr()
+    packed.codes.zero_()
+    assert not packed.dequantize().any()
+    for other in copies[:2]:
+        assert torch.equal(other.dequantize(), want)
 
 
 @pytest.mark.gpu
