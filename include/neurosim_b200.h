@@ -563,7 +563,7 @@ typedef struct nsb_matrix {
 
 /* out[t, :] = scale * table[tokens[t], :], rounded once; a zero row where a token lies
  * outside [0, table->rows).  `tokens`: out->rows int32 or int64 (`token_bytes` 4 or 8).
- * `out` has the table's type or float32.  One launch. */
+ * `out` has the table's type or float32, and shares no element with the table.  One launch. */
 NSB_API int nsb_stimulus_drive(const void* tokens, int32_t token_bytes, const nsb_matrix* table,
                                float scale, const nsb_matrix* out, void* stream);
 
@@ -670,7 +670,8 @@ typedef struct nsb_row_values {
  * of the row's largest out value, -1 where none is above -inf (NaN is never chosen).  Lengths are
  * clamped to [0, history_length]; history entries outside [0, vocabulary) are skipped. */
 typedef struct nsb_logits {
-  nsb_matrix logits, out;  /* [rows, vocabulary < 2^30], same type; out may be the logits themselves */
+  nsb_matrix logits, out;  /* [rows, vocabulary < 2^30], same type; out may be the logits themselves,
+                            * or share no element with them */
   const int32_t* history;  /* [rows, history_length] */
   int64_t history_length, history_stride;
   const int32_t* lengths;        /* [rows], NULL: history_length */

@@ -27,6 +27,20 @@ bool check_matrix(const nsb_matrix* m, nsb::Dense* d, const char* shape, const c
   return true;
 }
 
+// Whether two matrices of one element size share no element: apart in memory, or columns side by side in rows that
+// are the same distance apart.
+bool apart(const nsb::Dense& a, const nsb::Dense& b) {
+  if (a.rows == 0 || b.rows == 0) return true;
+  const auto bytes = [](const nsb::Dense& m, int64_t elements) { return static_cast<uintptr_t>(elements) * nsb::value_bytes(m.type); };
+  const auto from_a = reinterpret_cast<uintptr_t>(a.data), from_b = reinterpret_cast<uintptr_t>(b.data);
+  if (from_a + bytes(a, (a.rows - 1) * a.stride + a.cols) <= from_b || from_b + bytes(b, (b.rows - 1) * b.stride + b.cols) <= from_a)
+    return true;
+  const uintptr_t pitch = bytes(a, a.stride);
+  if (pitch != bytes(b, b.stride)) return false;
+  const uintptr_t ahead = from_b >= from_a ? (from_b - from_a) % pitch : (pitch - (from_a - from_b) % pitch) % pitch;
+  return ahead >= bytes(a, a.cols) && ahead + bytes(b, b.cols) <= pitch;
+}
+
 bool check_tokens(const void* tokens, int32_t bytes, int64_t n) {
   if (bytes != 4 && bytes != 8) return fail("tokens must be int32 or int64");
   if (n > 0 && (!tokens || reinterpret_cast<uintptr_t>(tokens) % bytes != 0)) return fail("tokens are required, aligned to their size");
@@ -91,6 +105,7 @@ int nsb_stimulus_drive(const void* tokens, int32_t token_bytes, const nsb_matrix
     return NSB_ERR_ARGUMENT;
   if (o.cols != t.cols) return nsb::set_error(NSB_ERR_ARGUMENT, "drive and table must have the same number of neurons");
   if (o.type != t.type && o.type != NSB_VALUE_F32) return nsb::set_error(NSB_ERR_ARGUMENT, "the drive has the table's type or float32");
+  if (!apart(t, o)) return nsb::set_error(NSB_ERR_ARGUMENT, "the drive must not overlap with the table");
   if (!check_tokens(tokens, token_bytes, o.rows)) return NSB_ERR_ARGUMENT;
   nsb::set_error(NSB_OK, "");
   if (o.rows == 0) return NSB_OK;
@@ -309,6 +324,8 @@ int nsb_adjust_logits(const nsb_logits* args, void* stream) {
     return NSB_ERR_ARGUMENT;
   if (a.out.rows != a.logits.rows || a.out.cols != a.logits.cols || a.out.type != a.logits.type)
     return nsb::set_error(NSB_ERR_ARGUMENT, "the output must have the logits' shape and type");
+  if (!(a.out.data == a.logits.data && (a.out.rows <= 1 || a.out.stride == a.logits.stride)) && !apart(a.logits, a.out))
+    return nsb::set_error(NSB_ERR_ARGUMENT, "the output must be the logits themselves, or not overlap with them");
   if (a.logits.cols >= kMost / 2) return nsb::set_error(NSB_ERR_ARGUMENT, "the vocabulary must be below 2^30");
   if (args->history_length < 0 || args->history_length >= kMost || (args->history_length > 0 && a.logits.rows > 0 && (!args->history || args->history_stride < 0)))
     return nsb::set_error(NSB_ERR_ARGUMENT, "the history must be [rows, length] int32");

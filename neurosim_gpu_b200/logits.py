@@ -63,7 +63,7 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
     vocabulary are skipped); ``lengths`` / ``prompt_lengths``: int32 [B] (default: L / 0);
     ``repetition`` (above 0), ``presence``, ``frequency``: numbers or float32 [B]; ``bias``: float32
     [V] or [B, V]; ``mask``: int32 [ceil(V / 32)] or [B, ceil(V / 32)], bit v % 32 of word v // 32
-    set where token v is allowed.  ``out`` may be ``logits``.  The choice is the lowest index of a
+    set where token v is allowed.  ``out`` may be ``logits``, or share no element with them.  The choice is the lowest index of a
     row's largest adjusted logit, -1 where nothing is above -inf; a NaN is never chosen.
 
     There is no backward pass: where gradients are recorded, an argument that requires one is refused.

@@ -122,6 +122,34 @@ def test_entry_point_refuses_bad_arguments():
     assert call(logits=empty, out=empty) == 0
 
 
+def test_entry_points_refuse_results_that_overlap_with_what_they_read():
+    lib = native.load_library()
+    p = 0x10000  # never read: the checks fail first
+
+    def adjust(out, logits=(0, 3, 100, 200)):
+        args = native._Logits()
+        args.logits, args.out = (native._Matrix(p + 4 * at, rows, cols, stride, 0) for at, rows, cols, stride in (logits, out))
+        args.repetition.scalar = 0.0  # what the last check refuses
+        assert lib.nsb_adjust_logits(ctypes.byref(args), None) == -1
+        return b"overlap" not in lib.nsb_last_error()
+
+    # The same matrix, before it, behind it, and the other columns of its rows.
+    for at, stride in ((0, 200), (-500, 200), (500, 200), (500, 100), (100, 200), (-100, 200), (300, 200), (-300, 200)):
+        assert adjust((at, 3, 100, stride)), (at, stride)
+    for at, stride in ((1, 200), (-1, 200), (99, 200), (-99, 200), (0, 201), (0, 100), (499, 100), (200, 200), (101, 200)):
+        assert not adjust((at, 3, 100, stride)), (at, stride)
+    assert adjust((0, 1, 100, 150), (0, 1, 100, 100)) and adjust((100, 1, 100, 150), (0, 1, 100, 100))
+    assert not adjust((99, 1, 100, 150), (0, 1, 100, 100))
+
+    def drive(at, kind=0):
+        table, out = native._Matrix(p, 10, 8, 8, 1 if kind == 1 else 0), native._Matrix(p + at, 4, 8, 8, kind)
+        assert lib.nsb_stimulus_drive(None, 8, ctypes.byref(table), 1.0, ctypes.byref(out), None) == -1
+        return b"overlap" not in lib.nsb_last_error()
+
+    assert drive(320) and drive(-128) and drive(160, 1)
+    assert not drive(316) and not drive(-124) and not drive(0) and not drive(158, 1)
+
+
 def test_function_refuses_cpu_tensors():
     with pytest.raises(ValueError, match="CUDA"):
         adjust_logits(torch.zeros(2, 8))
@@ -239,6 +267,19 @@ def test_strided_rows_in_place_and_graph(dtype):
     a.zero_(), b.zero_()
     graph.replay()
     assert torch.equal(a, want) and torch.equal(b, choice)
+
+
+@pytest.mark.gpu
+def test_results_beside_the_logits_and_over_them():
+    base = torch.randn(5, 90, generator=generator(6)).cuda()
+    logits, bias = base[:, :45], torch.ones(45, device="cuda")
+    want = logits + 1
+    for bad in (base[:, 1:46], base[:, 44:89], base.view(-1)[: 5 * 45].view(5, 45)):
+        with pytest.raises(RuntimeError, match="overlap"):
+            adjust_logits(logits, bias=bias, out=bad)
+    assert torch.equal(adjust_logits(logits, bias=bias, out=base[:, 45:]), want)  # the other half of each row
+    assert torch.equal(adjust_logits(logits, bias=bias, out=base[:, :45]), want)  # another tensor, the same elements
+    assert torch.equal(logits, want)
 
 
 @pytest.mark.gpu
