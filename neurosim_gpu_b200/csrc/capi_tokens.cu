@@ -41,6 +41,10 @@ bool apart(const nsb::Dense& a, const nsb::Dense& b) {
   return ahead >= bytes(a, a.cols) && ahead + bytes(b, b.cols) <= pitch;
 }
 
+bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+bool check_status(const int* status) { return aligned(status, 4) ? true : fail("the status word must be 4-byte aligned"); }
+
 bool check_tokens(const void* tokens, int32_t bytes, int64_t n) {
   if (bytes != 4 && bytes != 8) return fail("tokens must be int32 or int64");
   if (n > 0 && (!tokens || reinterpret_cast<uintptr_t>(tokens) % bytes != 0)) return fail("tokens are required, aligned to their size");
@@ -182,7 +186,7 @@ int nsb_nvfp4_product(const nsb_nvfp4* a, const nsb_nvfp4* b, const float* bias,
   if (x.cols != y.cols) return nsb::set_error(NSB_ERR_ARGUMENT, "the operands must have the same number of columns");
   if (y.rows < 1 || o.rows != x.rows || o.cols != y.rows)
     return nsb::set_error(NSB_ERR_ARGUMENT, "the product must be [a.rows, b.rows], b.rows >= 1");
-  if (!product_ok(x.rows, y.rows)) return NSB_ERR_ARGUMENT;
+  if (!product_ok(x.rows, y.rows) || !check_status(status)) return NSB_ERR_ARGUMENT;
   if (reinterpret_cast<uintptr_t>(bias) % 4 != 0) return nsb::set_error(NSB_ERR_ARGUMENT, "the bias must be 4-byte aligned");
   nsb::set_error(NSB_OK, "");
   if (x.rows == 0) return NSB_OK;
@@ -212,7 +216,7 @@ int nsb_nvfp4_readout(const nsb_matrix* state, const nsb_nvfp4* weight, const fl
   if (x.cols != w.cols) return nsb::set_error(NSB_ERR_ARGUMENT, "states and weights must have the same number of columns");
   if (w.rows < 1 || o.rows != x.rows || o.cols != w.rows)
     return nsb::set_error(NSB_ERR_ARGUMENT, "the output must be [state.rows, weight.rows], weight.rows >= 1");
-  if (!product_ok(x.rows, w.rows)) return NSB_ERR_ARGUMENT;
+  if (!product_ok(x.rows, w.rows) || !check_status(status)) return NSB_ERR_ARGUMENT;
   if (reinterpret_cast<uintptr_t>(bias) % 4 != 0) return nsb::set_error(NSB_ERR_ARGUMENT, "the bias must be 4-byte aligned");
   if (!check_workspace(workspace, workspace_bytes, nsb_nvfp4_readout_workspace_size(x.rows, x.cols), 16)) return NSB_ERR_WORKSPACE;
   nsb::set_error(NSB_OK, "");
@@ -243,7 +247,7 @@ int nsb_nvfp4_train_forward(const nsb_matrix* state, const nsb_matrix* weight, c
     return NSB_ERR_ARGUMENT;
   if (x.cols != w.cols || w.rows < 1 || o.rows != x.rows || o.cols != w.rows)
     return nsb::set_error(NSB_ERR_ARGUMENT, "states [M, K], weights [N >= 1, K] and output [M, N] do not fit together");
-  if (!product_ok(x.rows, w.rows)) return NSB_ERR_ARGUMENT;
+  if (!product_ok(x.rows, w.rows) || !check_status(status)) return NSB_ERR_ARGUMENT;
   if (reinterpret_cast<uintptr_t>(bias) % 4 != 0 || !largest || reinterpret_cast<uintptr_t>(largest) % 4 != 0)
     return nsb::set_error(NSB_ERR_ARGUMENT, "two words for the largest sizes are required; they and the bias must be 4-byte aligned");
   if (!check_workspace(workspace, workspace_bytes, nsb_nvfp4_train_workspace_size(x.rows, x.cols, w.rows), 16)) return NSB_ERR_WORKSPACE;
@@ -272,7 +276,7 @@ int nsb_nvfp4_train_backward(const nsb_matrix* state, const nsb_matrix* weight, 
   if (x.rows < 1 || w.rows < 1 || x.cols != w.cols || d.rows != x.rows || d.cols != w.rows ||
       (state_grad && (dx.rows != x.rows || dx.cols != x.cols)) || (weight_grad && (dw.rows != w.rows || dw.cols != w.cols)))
     return nsb::set_error(NSB_ERR_ARGUMENT, "states [M >= 1, K], weights [N >= 1, K], the output's gradient [M, N] and the gradients do not fit together");
-  if (!product_ok(x.rows, w.rows) || !product_ok(x.cols, x.cols)) return NSB_ERR_ARGUMENT;
+  if (!product_ok(x.rows, w.rows) || !product_ok(x.cols, x.cols) || !check_status(status)) return NSB_ERR_ARGUMENT;
   if (!largest || reinterpret_cast<uintptr_t>(largest) % 4 != 0 || reinterpret_cast<uintptr_t>(bias_grad) % 4 != 0)
     return nsb::set_error(NSB_ERR_ARGUMENT, "the largest sizes of the forward call are required; they and the bias's gradient must be 4-byte aligned");
   if (!check_workspace(workspace, workspace_bytes, nsb_nvfp4_train_workspace_size(x.rows, x.cols, w.rows), 16)) return NSB_ERR_WORKSPACE;
@@ -332,6 +336,10 @@ int nsb_adjust_logits(const nsb_logits* args, void* stream) {
   if ((args->bias && args->bias_stride < 0) || (args->mask && args->mask_stride < 0) ||
       args->repetition.stride < 0 || args->presence.stride < 0 || args->frequency.stride < 0)
     return nsb::set_error(NSB_ERR_ARGUMENT, "strides must not be negative");
+  if (!aligned(args->history, 4) || !aligned(args->lengths, 4) || !aligned(args->prompt_lengths, 4) || !aligned(args->bias, 4) ||
+      !aligned(args->mask, 4) || !aligned(args->choice, 8) || !aligned(args->repetition.data, 4) ||
+      !aligned(args->presence.data, 4) || !aligned(args->frequency.data, 4))
+    return nsb::set_error(NSB_ERR_ARGUMENT, "history, lengths, penalties, bias, mask and choice must be aligned to their elements");
   if (!args->repetition.data && !(args->repetition.scalar > 0.0f))
     return nsb::set_error(NSB_ERR_ARGUMENT, "the repetition penalty must be above 0");
   a.history = args->history;

@@ -150,6 +150,20 @@ def test_entry_points_refuse_results_that_overlap_with_what_they_read():
     assert not drive(316) and not drive(-124) and not drive(0) and not drive(158, 1)
 
 
+def test_entry_point_refuses_addresses_that_are_not_aligned():
+    lib = native.load_library()
+    p = 0x10000  # never read: the checks fail first
+    for name, step in (("history", 2), ("lengths", 1), ("prompt_lengths", 2), ("bias", 2), ("mask", 3), ("choice", 4), ("repetition", 2),
+                       ("presence", 1), ("frequency", 2)):
+        args = native._Logits()
+        args.logits = args.out = native._Matrix(p, 2, 100, 100, 0)
+        args.repetition.scalar = 1.0
+        args.history, args.history_length = p, 5
+        setattr(args, name, native._RowValues(p + step, 1, 1.0) if isinstance(getattr(args, name), native._RowValues) else p + step)
+        assert lib.nsb_adjust_logits(ctypes.byref(args), None) == -1, name
+        assert b"aligned" in lib.nsb_last_error(), name
+
+
 def test_function_refuses_cpu_tensors():
     with pytest.raises(ValueError, match="CUDA"):
         adjust_logits(torch.zeros(2, 8))

@@ -424,6 +424,18 @@ def test_waits_that_run_out_report_and_leave_the_context_usable(m, n, k):
     assert torch.equal(out.cpu().double(), x @ y.t())
 
 
+def test_products_refuse_a_status_word_that_is_not_aligned():
+    lib = native.load_library()
+    p, status = 0x1000, 0x1002  # never read: the checks fail first
+    state, weight, out = (ctypes.byref(native._Matrix(p, *s, s[1], 0)) for s in ((4, 16), (6, 16), (4, 6)))
+    a, b = (ctypes.byref(native._Nvfp4(rows, 16, p, 16, p, p, 1)) for rows in (4, 6))
+    for result in (lib.nsb_nvfp4_product(a, b, None, out, status, None),
+                   lib.nsb_nvfp4_readout(state, b, None, out, p, 2**40, status, None),
+                   lib.nsb_nvfp4_train_forward(state, weight, None, out, p, p, 2**40, status, None),
+                   lib.nsb_nvfp4_train_backward(state, weight, out, p, state, weight, None, p, 2**40, status, None)):
+        assert result == -1 and b"status" in lib.nsb_last_error()
+
+
 def test_status_needs_a_place_for_the_code():
     assert native.load_library().nsb_nvfp4_product_status(None, None) == -1
 
