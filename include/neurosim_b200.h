@@ -614,8 +614,9 @@ NSB_API int nsb_nvfp4_dequantize(const nsb_nvfp4* value, const nsb_matrix* out, 
 NSB_API int nsb_nvfp4_product(const nsb_nvfp4* a, const nsb_nvfp4* b, const float* bias,
                               const nsb_matrix* out, int* status, void* stream);
 
-/* How often the bounded waits of later products of this process poll before they give up: below 0 the
- * default.  For tests: with 0 every product gives up, and leaves its output as it was. */
+/* For tests: later products of this process issue nothing to the tensor cores, so that the waits for that run
+ * out, after `polls` polls (in steps of 256); they report it and leave their output as it was.  Below 0: the
+ * default, products as usual. */
 NSB_API void nsb_nvfp4_product_wait_limit(int32_t polls);
 
 /* *code (host) = the code that products with no status word of their own have left on the current device

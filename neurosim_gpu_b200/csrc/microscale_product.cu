@@ -82,7 +82,7 @@ struct ProductArgs {
   int64_t scale_tiles;  // 512-byte tiles per 128 rows
   int32_t k_tiles, split;
   int32_t lane_tiles, column_tiles;  // lane tiles of 128, of pairs 256
-  int polls;  // of a bounded wait
+  int polls;  // of a bounded wait; below kBarrierPolls no product is issued, and the waits for them run out
   bool lane_ready;  // the operand along the lanes was complete before the kernel ahead of this one started
   int* status;
 };
@@ -177,7 +177,8 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
   tcgen05_fence_after();
   const uint32_t tmem = h.tmem;
 
-  int loads = 0;  // K tiles that warp 0 has asked for
+  int loads = 0;         // K tiles that warp 0 has asked for
+  bool drained = false;  // warp 1 has waited for its products
   if (warp == 0) {  // loads
     Ring<S::kStages> ring;
     int ahead = 0;
@@ -245,7 +246,7 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
   } else if (warp == 1) {  // products
     Ring<S::kStages> ring;
     int t = 0;
-    bool ok = true;
+    bool ok = a.polls == kBarrierPolls;
     const uint64_t lane_codes = swizzled_descriptor(shared_addr(stages));
     const uint64_t column_codes = swizzled_descriptor(shared_addr(stages + kLaneBytes));
     const uint64_t scales = plain_descriptor(shared_addr(stages + kLaneBytes + S::kColumnBytes));
@@ -290,13 +291,17 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
         __syncwarp();
       }
     }
+    if (*aborted) {
+      if (elect_one()) mma_commit<kPair>(&h.drained);
+      barrier_drain(&h.drained, 0);
+      drained = true;
+    }
   } else {  // results: a warp reads lanes 32 (warp % 4) ... of its columns
     grid_wait();  // the scales may be the kernel's ahead, and what it reads may lie where this one writes
     const int quarter = warp & 3, slot = threadIdx.x - 64;
     const int part = (warp - 2) / 4 * S::kOutColumns;  // first column
     int t = 0;
     bool ok = true;  // once a wait has given up, the tiles are walked for their barriers alone
-    const long long sum_polls = a.polls * (1ll + (k1 - k0) / 1024);  // the wait for all of a tile's products
     for (int tile = first; tile < tiles; tile += step, ++t) {
       int lt, ct;
       place(a, tile, &lt, &ct);
@@ -315,7 +320,7 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
       const bool in = row < a.lane.rows;
       const float row_scale = in ? __ldg(a.lane.scale + (a.lane.per_row ? row : 0)) : 0.0f;
       const float row_bias = in && a.lane.bias ? __ldg(a.lane.bias + row) : 0.0f;
-      if (ok && !barrier_wait(&h.sum_full[b], use & 1, aborted, sum_polls)) {
+      if (ok && !barrier_wait(&h.sum_full[b], use & 1, aborted, a.polls)) {
         if (lane == 0) give_up(a, aborted, 4);
         ok = false;
       }
@@ -361,7 +366,7 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
   if (*aborted) {  // by any role: no copy may land and no product run after the CTA has gone
     if (warp == 0)
       for (int u = max(0, loads - S::kStages); u < loads; ++u) barrier_drain(&h.full[u % S::kStages], (u / S::kStages) & 1);
-    if (warp == 1 && issues) {
+    if (warp == 1 && issues && !drained) {
       if (elect_one()) mma_commit<kPair>(&h.drained);
       barrier_drain(&h.drained, 0);
     }
@@ -500,7 +505,7 @@ cudaError_t launch(const Nvfp4& lane, const Nvfp4& column, ProductArgs a, int sm
 
 }  // namespace
 
-void set_product_polls(int polls) { g_polls.store(polls < 0 ? kBarrierPolls : polls, std::memory_order_relaxed); }
+void set_product_polls(int polls) { g_polls.store(polls < 0 ? kBarrierPolls : std::min(polls, kBarrierPolls - 1), std::memory_order_relaxed); }
 
 cudaError_t take_product_status(int* code, cudaStream_t stream) {
   void* word = nullptr;

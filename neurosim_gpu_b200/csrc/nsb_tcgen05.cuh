@@ -73,16 +73,16 @@ __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// Polls before a wait gives up (tens of milliseconds at the least).
+// Polls before a wait gives up: 4 us each, 17 s (a sum over 2^31 columns takes about two).
 constexpr int kBarrierPolls = 1 << 22;
 
-// Waits for the phase `parity` of `bar`, `polls` times at most; gives up at once when another role of the CTA has (`*aborted`).
-__device__ __forceinline__ bool barrier_wait(uint64_t* bar, uint32_t parity, volatile int* aborted, long long polls) {
-  for (long long i = 0; i < polls; ++i) {
+// Waits for the phase `parity` of `bar`.  At every 256th poll it gives up where another role of the CTA has
+// (`*aborted`), or after `polls`.
+__device__ __forceinline__ bool barrier_wait(uint64_t* bar, uint32_t parity, volatile int* aborted, int polls) {
+  for (int i = 1;; ++i) {
     if (barrier_try(bar, parity)) return true;
-    if ((i & 255) == 255 && *aborted) return false;
+    if ((i & 255) == 0 && (*aborted || i >= polls)) return false;
   }
-  return false;
 }
 
 // After a wait has given up: for work in flight, which ends by itself; bounded all the same.
