@@ -19,8 +19,8 @@
 // Large products run on pairs of CTAs (tcgen05 cta_group::2): a tile of 256 lanes x 256 columns, of which
 // each CTA holds 128 lanes' sums and loads its 128 lanes' codes and half of the columns'.  A CTA of its
 // own takes 54 KB from L2 per K tile, at 64 bytes a cycle longer than its products do (860 cycles against
-// 512 of the tensor core); one of a pair takes 38 KB.  The first CTA issues for both, after the second
-// has passed on that its own loads are in.
+// 512 of the tensor core); one of a pair takes 38 KB.  The first CTA issues for both: the loads of both,
+// which are tensor copies throughout, complete on its barriers.
 //
 // Few rows are bound by reading the weights: 1 x 32,000 x 4,096 15.3 us, 4.8 TB/s.  Many are bound by the tensor
 // cores, 76 % of the time active: 8,192 x 8,192 x 4,096 109 us, 5.0 PFLOP/s; x 32,768 764 us, 5.8 PFLOP/s.
@@ -89,10 +89,10 @@ struct ProductArgs {
 
 struct Header {
   uint64_t full[8], empty[8];
-  uint64_t peer_full[8];  // of a pair's first CTA: the second's loads
   uint64_t sum_full[2], sum_empty[2], drained;
   uint32_t tmem;
   int aborted;
+  int peer_aborted, peer_loads;  // of a pair: what the other CTA leaves as its roles end
   alignas(16) float scale[256];  // of the tile's columns
   alignas(16) float bias[256];
 };
@@ -118,6 +118,16 @@ __device__ __forceinline__ float scaled(float sum, float lane_scale, float colum
   return __fadd_rn(__fmul_rn(__fmul_rn(sum, lane_scale), column_scale), bias);
 }
 
+// Boxes of both operands' codes; of a pair also rows of 2,048 bytes of their block scales.
+template <bool kPair>
+struct Maps {
+  CUtensorMap lane, column;
+};
+template <>
+struct Maps<true> {
+  CUtensorMap lane, column, lane_scales, column_scales;
+};
+
 // A position in the ring of stages and the parity of its round.
 template <int kStages>
 struct Ring {
@@ -133,8 +143,7 @@ struct Ring {
 
 template <typename O, int kColumns, bool kPair>
 __global__ void __launch_bounds__(Shape<kColumns, kPair>::kThreads, 1)
-product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_constant__ CUtensorMap column_map,
-               const __grid_constant__ ProductArgs a) {
+product_kernel(const __grid_constant__ Maps<kPair> maps, const __grid_constant__ ProductArgs a) {
   using S = Shape<kColumns, kPair>;
   extern __shared__ __align__(1024) uint8_t shared[];
   Header& h = *reinterpret_cast<Header*>(shared);
@@ -160,7 +169,6 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
     for (int s = 0; s < S::kStages; ++s) {
       barrier_init(&h.full[s], 1);
       barrier_init(&h.empty[s], 1);
-      barrier_init(&h.peer_full[s], 1);
     }
     for (int s = 0; s < 2; ++s) {
       barrier_init(&h.sum_full[s], 1);
@@ -181,6 +189,36 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
   bool drained = false;  // warp 1 has waited for its products
   if (warp == 0) {  // loads
     Ring<S::kStages> ring;
+    // One thread: the lanes' share of a stage, which its barrier then expects whole (a pair's both halves).
+    auto load_lanes = [&](int stage, int lane_tile, int k) {
+      uint8_t* to = stages + stage * S::kStageBytes;
+      uint64_t* full = &h.full[stage];
+      if (issues) barrier_arrive_expect(full, (kPair ? 2 : 1) * S::kStageBytes);
+      if constexpr (kPair) {
+        const uint32_t bar = remote_address(shared_addr(full), 0);
+        load_box_pair(to, &maps.lane, k * kTileBytes, lane_block(lane_tile) * kLanes, bar);
+        load_row_pair(to + kLaneBytes + S::kColumnBytes, &maps.lane_scales, k, static_cast<int>(lane_scale_block(lane_tile)), bar);
+      } else {
+        load_box(to, &maps.lane, k * kTileBytes, lane_block(lane_tile) * kLanes, full);
+        load_bytes(to + kLaneBytes + S::kColumnBytes, a.lane.block_scales + (lane_scale_block(lane_tile) * a.scale_tiles + static_cast<int64_t>(k) * 4) * 512,
+                   kScaleBytes, full);
+      }
+    };
+    auto load_columns = [&](int stage, int column_tile, int k) {
+      uint8_t* to = stages + stage * S::kStageBytes + kLaneBytes;
+      uint64_t* full = &h.full[stage];
+      const uint32_t bar = kPair ? remote_address(shared_addr(full), 0) : 0;
+      if constexpr (kPair) load_box_pair(to, &maps.column, k * kTileBytes, column_tile * kColumns + rank * S::kColumnRows, bar);
+      else load_box(to, &maps.column, k * kTileBytes, column_tile * kColumns, full);
+      to += S::kColumnBytes;
+#pragma unroll
+      for (int c = 0; c < S::kBlocks; ++c) {
+        // A tile that ends before its second block of 128 rows loads the first one again.
+        const int64_t ahead_of = static_cast<int64_t>(column_tile) * S::kBlocks + c, block = ahead_of * 128 < a.column.rows ? ahead_of : 0;
+        if constexpr (kPair) load_row_pair(to + kScaleBytes * (1 + c), &maps.column_scales, k, static_cast<int>(block), bar);
+        else load_bytes(to + kScaleBytes * (1 + c), a.column.block_scales + (block * a.scale_tiles + static_cast<int64_t>(k) * 4) * 512, kScaleBytes, full);
+      }
+    };
     int ahead = 0;
     bool ok = true;
     if (a.lane_ready && first < tiles) {  // its first stages' share while the kernel ahead still runs
@@ -188,62 +226,27 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
       place(a, first, &lt, &ct);
       ahead = min(S::kStages, k1 - k0);
       if (elect_one())
-        for (int s = 0; s < ahead; ++s) {
-          uint8_t* to = stages + s * S::kStageBytes;
-          barrier_arrive_expect(&h.full[s], S::kStageBytes);
-          load_box(to, &lane_map, (k0 + s) * kTileBytes, lane_block(lt) * kLanes, &h.full[s]);
-          load_bytes(to + kLaneBytes + S::kColumnBytes, a.lane.block_scales + (lane_scale_block(lt) * a.scale_tiles + (k0 + s) * 4) * 512,
-                     kScaleBytes, &h.full[s]);
-        }
+        for (int s = 0; s < ahead; ++s) load_lanes(s, lt, k0 + s);
       __syncwarp();
     }
     grid_wait();
     for (int tile = first; ok && tile < tiles; tile += step) {
       int lt, ct;
       place(a, tile, &lt, &ct);
-      const uint8_t* lane_scales = a.lane.block_scales + lane_scale_block(lt) * a.scale_tiles * 512;
-      const uint8_t* column_scales[S::kBlocks];
-#pragma unroll
-      for (int c = 0; c < S::kBlocks; ++c) {
-        // A tile that ends before its second block of 128 rows loads the first one again.
-        const int64_t block = static_cast<int64_t>(ct) * S::kBlocks + c;
-        column_scales[c] = a.column.block_scales + (block * 128 < a.column.rows ? block : 0) * a.scale_tiles * 512;
-      }
       for (int k = k0; k < k1; ++k, ++loads, ring.next()) {
-        uint64_t* full = &h.full[ring.stage];
         if (ring.round > 0 && !barrier_wait(&h.empty[ring.stage], (ring.round - 1) & 1, aborted, a.polls)) {
           ok = false;
           break;
         }
         if (elect_one()) {
-          uint8_t* to = stages + ring.stage * S::kStageBytes;
-          const int64_t scale_offset = static_cast<int64_t>(k) * kScaleBytes;  // beyond 2^31 from 2^20 K tiles on
-          if (loads >= ahead) {
-            barrier_arrive_expect(full, S::kStageBytes);
-            load_box(to, &lane_map, k * kTileBytes, lane_block(lt) * kLanes, full);
-            load_bytes(to + kLaneBytes + S::kColumnBytes, lane_scales + scale_offset, kScaleBytes, full);
-          }
-          load_box(to + kLaneBytes, &column_map, k * kTileBytes, ct * kColumns + (kPair ? rank * S::kColumnRows : 0), full);
-          to += kLaneBytes + S::kColumnBytes;
-#pragma unroll
-          for (int c = 0; c < S::kBlocks; ++c)
-            load_bytes(to + kScaleBytes * (1 + c), column_scales[c] + scale_offset, kScaleBytes, full);
+          if (loads >= ahead) load_lanes(ring.stage, lt, k);
+          load_columns(ring.stage, ct, k);
         }
         __syncwarp();
       }
     }
     if (!ok && lane == 0) give_up(a, aborted, 1);
-  } else if (warp == 1 && !issues) {  // the pair's second CTA: its loads are in
-    Ring<S::kStages> ring;
-    bool ok = true;
-    for (int tile = first; ok && tile < tiles; tile += step)
-      for (int k = k0; ok && k < k1; ++k, ring.next()) {
-        ok = barrier_wait(&h.full[ring.stage], ring.round & 1, aborted, a.polls);
-        if (ok && elect_one()) barrier_arrive_at(&h.peer_full[ring.stage], 0);
-        __syncwarp();
-      }
-    if (!ok && lane == 0) give_up(a, aborted, 5);
-  } else if (warp == 1) {  // products
+  } else if (warp == 1 && issues) {  // products
     Ring<S::kStages> ring;
     int t = 0;
     bool ok = a.polls == kBarrierPolls;
@@ -263,8 +266,7 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
       const uint32_t instruction = nvfp4_instruction(kPair ? 2 * kLanes : kLanes, kPair ? kColumns : min(kColumns, (a.column.rows - ct * kColumns + 15) / 16 * 16));
       const uint32_t sum = tmem + b * kColumns;
       for (int k = k0; k < k1; ++k, ring.next()) {
-        if (!barrier_wait(&h.full[ring.stage], ring.round & 1, aborted, a.polls) ||
-            (kPair && !barrier_wait(&h.peer_full[ring.stage], ring.round & 1, aborted, a.polls))) {
+        if (!barrier_wait(&h.full[ring.stage], ring.round & 1, aborted, a.polls)) {
           if (lane == 0) give_up(a, aborted, 3);
           ok = false;
           break;
@@ -296,7 +298,7 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
       barrier_drain(&h.drained, 0);
       drained = true;
     }
-  } else {  // results: a warp reads lanes 32 (warp % 4) ... of its columns
+  } else if (warp > 1) {  // results: a warp reads lanes 32 (warp % 4) ... of its columns
     grid_wait();  // the scales may be the kernel's ahead, and what it reads may lie where this one writes
     const int quarter = warp & 3, slot = threadIdx.x - 64;
     const int part = (warp - 2) / 4 * S::kOutColumns;  // first column
@@ -364,16 +366,36 @@ product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_consta
   tcgen05_fence_before();
   __syncthreads();
   if (*aborted) {  // by any role: no copy may land and no product run after the CTA has gone
-    if (warp == 0)
-      for (int u = max(0, loads - S::kStages); u < loads; ++u) barrier_drain(&h.full[u % S::kStages], (u / S::kStages) & 1);
     if (warp == 1 && issues && !drained) {
       if (elect_one()) mma_commit<kPair>(&h.drained);
       barrier_drain(&h.drained, 0);
     }
+    if (!kPair && warp == 0)
+      for (int u = max(0, loads - S::kStages); u < loads; ++u) barrier_drain(&h.full[u % S::kStages], (u / S::kStages) & 1);
     __syncthreads();
   }
   if (kPair) {
+    if (threadIdx.x == 0) {
+      remote_store(&h.peer_aborted, rank ^ 1, *aborted);
+      remote_store(&h.peer_loads, rank ^ 1, loads);
+    }
+    __syncwarp();
     cluster_barrier();  // neither CTA goes while the other may still arrive on its barriers or use its memory
+    if (*aborted || h.peer_aborted) {
+      if (warp == 0 && issues) {  // the copies of both: a K tile that one of them has not asked for lacks its share
+        const int other = h.peer_loads, most = max(loads, other);
+        for (int u = max(0, most - S::kStages); u < most; ++u) {
+          uint64_t* full = &h.full[u % S::kStages];
+          if (elect_one()) {
+            if (u >= loads) barrier_arrive_expect(full, S::kStageBytes);
+            else if (u >= other) barrier_forgo(full, S::kStageBytes);
+          }
+          __syncwarp();
+          barrier_drain(full, (u / S::kStages) & 1);
+        }
+      }
+      cluster_barrier();
+    }
   } else if (a.split > 1) {
     cluster_barrier();
     int lt, ct;
@@ -462,6 +484,17 @@ bool map_codes(const Nvfp4& m, int rows, CUtensorMap* map) {
                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Rows of 2,048 bytes, the block scales of 128 rows and 256 columns: [ceil(rows / 128), ceil(cols / 256), 256 words of 8 bytes].
+bool map_scales(const Nvfp4& m, CUtensorMap* map) {
+  const auto across = static_cast<cuuint64_t>(block_scale_tiles(m.cols) / 4);
+  const cuuint64_t size[3] = {kScaleBytes / 8, across, static_cast<cuuint64_t>((m.rows + 127) / 128)};
+  const cuuint64_t stride[2] = {kScaleBytes, kScaleBytes * across};
+  const cuuint32_t box[3] = {kScaleBytes / 8, 1, 1}, one[3] = {1, 1, 1};
+  return encoder() && encoder()(map, CU_TENSOR_MAP_DATA_TYPE_UINT64, 3, m.block_scales, size, stride, box, one,
+                                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename O, int kColumns, bool kPair = false>
 cudaError_t launch(const Nvfp4& lane, const Nvfp4& column, ProductArgs a, int sm_count, cudaStream_t stream) {
   using S = Shape<kColumns, kPair>;
@@ -470,8 +503,11 @@ cudaError_t launch(const Nvfp4& lane, const Nvfp4& column, ProductArgs a, int sm
   a.column_tiles = (a.column.rows + kColumns - 1) / kColumns;
   const int64_t tiles = static_cast<int64_t>(a.lane_tiles) * a.column_tiles;
   if (tiles > 0x3fffffff) return cudaErrorInvalidConfiguration;
-  CUtensorMap lane_map, column_map;
-  if (!map_codes(lane, kLanes, &lane_map) || !map_codes(column, S::kColumnRows, &column_map)) return cudaErrorInvalidValue;
+  Maps<kPair> maps;
+  if (!map_codes(lane, kLanes, &maps.lane) || !map_codes(column, S::kColumnRows, &maps.column)) return cudaErrorInvalidValue;
+  if constexpr (kPair) {
+    if (!map_scales(lane, &maps.lane_scales) || !map_scales(column, &maps.column_scales)) return cudaErrorInvalidValue;
+  }
   static SharedLimit limit;
   cudaError_t err = limit.raise(product_kernel<O, kColumns, kPair>, S::kShared);
   if (err != cudaSuccess) return err;
@@ -500,7 +536,7 @@ cudaError_t launch(const Nvfp4& lane, const Nvfp4& column, ProductArgs a, int sm
   attributes[1].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attributes;
   config.numAttrs = 2;
-  return cudaLaunchKernelEx(&config, product_kernel<O, kColumns, kPair>, lane_map, column_map, a);
+  return cudaLaunchKernelEx(&config, product_kernel<O, kColumns, kPair>, maps, a);
 }
 
 }  // namespace

@@ -21,11 +21,14 @@ __device__ __forceinline__ bool elect_one() {
 // Until the kernels ahead in the stream are complete (a launch that may overlap them).
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// One float32, or four, of CTA `rank`'s shared memory in the cluster, where this CTA's `address` would be.
+// A word, one float32, or four, of CTA `rank`'s shared memory in the cluster, where this CTA's `address` would be.
 __device__ __forceinline__ uint32_t remote_address(uint32_t address, int rank) {
   uint32_t remote;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(address), "r"(rank));
   return remote;
+}
+__device__ __forceinline__ void remote_store(int* own, int rank, int v) {
+  asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(remote_address(shared_addr(own), rank)), "r"(v) : "memory");
 }
 __device__ __forceinline__ void remote_load(uint32_t address, int rank, float (&v)[1]) {
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[0]) : "r"(remote_address(address, rank)) : "memory");
@@ -60,13 +63,15 @@ __device__ __forceinline__ bool barrier_try(uint64_t* bar, uint32_t parity) {
   return done != 0;
 }
 
-// Arrives on the barrier that lies at `bar` in the shared memory of the cluster's CTA `rank`.  What it
-// tells of are copies and tensor-core work, which complete on barriers of their own before: no fence for
-// plain memory accesses (release.cluster), which takes the relay of a pair about a microsecond.
+// Arrives on the barrier that lies at `bar` in the shared memory of the cluster's CTA `rank`.  It tells that the
+// warp's tensor memory has been read: tcgen05.wait::ld and the tcgen05 fences order that, no plain memory access.
 __device__ __forceinline__ void barrier_arrive_at(uint64_t* bar, int rank) {
-  uint32_t remote;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(shared_addr(bar)), "r"(rank));
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(remote_address(shared_addr(bar), rank)) : "memory");
+}
+
+// Counts `bytes` as arrived that no copy will bring.
+__device__ __forceinline__ void barrier_forgo(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(shared_addr(bar)), "r"(bytes) : "memory");
 }
 
 __device__ __forceinline__ void cluster_barrier() {
@@ -100,6 +105,23 @@ __device__ __forceinline__ void load_box(void* to, const void* map, int x, int y
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
           shared_addr(to)),
       "l"(map), "r"(x), "r"(y), "r"(shared_addr(bar))
+      : "memory");
+}
+
+// The same of a pair's CTA, to its own shared memory, and a box of 2,048 bytes at the start of a row of a
+// three-dimensional tensor.  `bar`: an address in the cluster's shared memory, so the barrier may be the other CTA's.
+__device__ __forceinline__ void load_box_pair(void* to, const void* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+          shared_addr(to)),
+      "l"(map), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void load_row_pair(void* to, const void* map, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          shared_addr(to)),
+      "l"(map), "r"(0), "r"(y), "r"(z), "r"(bar)
       : "memory");
 }
 
