@@ -206,6 +206,20 @@ def test_quantize(dtype, rows, columns):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("offset,odd", [(0, 0), (3, 1)])
+@pytest.mark.parametrize("rows,columns", [(300, 4104), (2, 132_000), (3, 166_003), (129, 9001), (5, 70_017)])
+def test_quantize_rows_longer_than_the_registers_hold(dtype, offset, odd, rows, columns):
+    """Their last blocks are read twice, for the row's largest size and for the codes; the largest lies there."""
+    stride = (columns + 15) // 16 * 16 + odd
+    base = torch.randn(offset + rows * stride, generator=generator(rows)).to(dtype)
+    x = base.as_strided((rows, columns), (stride, 1), offset)
+    x[::2, -1] = 37.0
+    x[1::2, -40] = -41.0
+    check_packed(quantize_nvfp4(base.cuda().as_strided((rows, columns), (stride, 1), offset)), x, "row")
+
+
+@pytest.mark.gpu
 def test_quantize_strides_ties_and_small_values():
     g = generator(3)
     base = torch.randn(60 * 70, generator=g)
