@@ -109,9 +109,9 @@ class Nvfp4Matrix:
         """The values the codes stand for: level * (block scale * scale), rounded to ``dtype``."""
         if dtype not in VALUE_TYPES:
             raise ValueError("dtype must be float32, float16 or bfloat16")
-        refuse_gradients("dequantize takes no gradients: its scale requires one", self.scale)
-        rows, columns = self.shape
-        out = self.scale.new_empty((rows, columns), dtype=dtype)
+        refuse_gradients("dequantize takes no gradients: its scale requires one", self._scale)
+        rows, columns = self._view.rows, self._view.cols
+        out = self._scale.new_empty((rows, columns), dtype=dtype)
         result = _Matrix(out.data_ptr(), rows, columns, columns, VALUE_TYPES[dtype])
         token_call(out, load_library().nsb_nvfp4_dequantize, ctypes.byref(self._view),
                    ctypes.byref(result))
@@ -175,9 +175,9 @@ def nvfp4_product(a: Nvfp4Matrix, b: Nvfp4Matrix, *, bias: torch.Tensor | None =
     alone (the same call gives the same bits).  ``out`` receives it where given (contiguous rows).
     Nothing here takes a gradient (:func:`nvfp4_readout` does).
     """
-    refuse_gradients("nvfp4_product takes no gradients: use nvfp4_readout, or detached tensors", bias, out, a.scale, b.scale)
-    m, n, device = a.rows, b.rows, a.scale.get_device()
-    if a.columns != b.columns or device != b.scale.get_device():
+    refuse_gradients("nvfp4_product takes no gradients: use nvfp4_readout, or detached tensors", bias, out, a._scale, b._scale)
+    m, n, device = a._view.rows, b._view.rows, a._scale.get_device()
+    if a._columns != b._columns or device != b._scale.get_device():
         raise ValueError("the operands must have the same number of columns and the same device")
     if n < 1:
         raise ValueError("the second operand needs at least one row")
@@ -186,7 +186,7 @@ def nvfp4_product(a: Nvfp4Matrix, b: Nvfp4Matrix, *, bias: torch.Tensor | None =
     if out is None:
         if dtype not in VALUE_TYPES:
             raise ValueError("dtype must be float32, float16 or bfloat16")
-        out = a.scale.new_empty((m, n), dtype=dtype)
+        out = a._scale.new_empty((m, n), dtype=dtype)
     elif out.shape != (m, n) or out.dtype != dtype or out.get_device() != device:
         raise ValueError("out must be [M, N] of the given dtype on the operands' device")
     result = dense_matrix(out, "out")
@@ -207,8 +207,8 @@ def _readout(state: torch.Tensor, weight: Nvfp4Matrix, bias: torch.Tensor | None
              dtype: torch.dtype) -> torch.Tensor:
     """[M, K] states through packed weights in one call of the library."""
     view = dense_matrix(state, "state")
-    rows, columns, n, device = view.rows, view.cols, weight.rows, state.get_device()
-    if weight.scale.get_device() != device or n < 1:
+    rows, columns, n, device = view.rows, view.cols, weight._view.rows, state.get_device()
+    if weight._scale.get_device() != device or n < 1:
         raise ValueError("weights must have at least one row and be on the states' device")
     _check_bias(bias, n, device)
     out = state.new_empty((rows, n), dtype=dtype)
@@ -288,10 +288,10 @@ def nvfp4_readout(state: torch.Tensor, weight: Nvfp4Matrix | torch.Tensor,
     if dtype not in VALUE_TYPES:
         raise ValueError("dtype must be float32, float16 or bfloat16")
     packed = isinstance(weight, Nvfp4Matrix)
-    scale = weight.scale if packed else None
+    scale = weight._scale if packed else None
     refuse_tangents("nvfp4_readout has no forward-mode derivative", state, scale if packed else weight, bias)
     shape = state.shape
-    if not shape or shape[-1] != (weight.columns if packed else weight.shape[-1]):
+    if not shape or shape[-1] != (weight._columns if packed else weight.shape[-1]):
         raise ValueError("states must be [..., K] for weights [N_out, K]")
     flat = state if len(shape) == 2 else state.reshape(-1, shape[-1])
     row_stride, stride = flat.stride()

@@ -349,14 +349,10 @@ def dense_matrix(value: torch.Tensor, name: str) -> _Matrix:
     return _Matrix(value.data_ptr(), rows, cols, row_stride if row_stride > cols else cols, kind)
 
 
-# Below 0 outside torch's forward-mode levels, where no tensor has a tangent.
-_forward_level = (lambda: forward_ad._current_level) if hasattr(forward_ad, "_current_level") else (lambda: 0)
-
-
 def refuse_tangents(message: str, *values) -> None:
     """Raise where one of the values is a dual tensor of forward-mode differentiation, whose tangent the
     call would drop."""
-    if _forward_level() >= 0:
+    if getattr(forward_ad, "_current_level", 0) >= 0:  # below: outside torch's forward mode, no tensor has one
         for value in values:
             if isinstance(value, torch.Tensor) and forward_ad.unpack_dual(value).tangent is not None:
                 raise ValueError(message)
@@ -366,7 +362,7 @@ def refuse_gradients(message: str, *values) -> None:
     """Raise where one of the values requires a gradient or has a tangent, which the call would drop."""
     if torch.is_grad_enabled():
         for value in values:
-            if isinstance(value, torch.Tensor) and value.requires_grad:
+            if getattr(value, "requires_grad", False):
                 raise ValueError(message)
     refuse_tangents(message, *values)
 
