@@ -493,7 +493,9 @@ join_sums_kernel(const float* sums, int64_t parts, int64_t cols, float* out) {
   out[c] = sum;
 }
 
-// Rows per partial sum: short enough to fill the GPU, and at most 64 parts.
+// Rows per partial sum: short enough to fill the GPU, and at most 64 parts, which one thread a column adds up.  At least
+// 64 rows: 256 x 50,000 f32 12.4 us, with 16 18.6, with 256 12.5 (488 x 25 f32: 3.5, 5.7 and 4.5).  64 parts:
+// 65,536 x 64 f32 14 us, 16 parts 39; 8,192 x 8,192 bf16 28 us, 16 parts 25, 256 parts 34.
 int64_t sum_span(int64_t rows) { return std::max<int64_t>(64, (rows + 63) / 64); }
 
 unsigned ceil_div(int64_t a, int64_t b) { return static_cast<unsigned>((a + b - 1) / b); }
@@ -511,11 +513,15 @@ cudaError_t amax_pass(Dense x, bool columns, unsigned int* amax, cudaStream_t st
   if ((err = device_info(&info)) != cudaSuccess) return err;
   if (columns) {
     const unsigned across = ceil_div(x.cols, 32 * P);
+    // Eight CTAs an SM, each with 64 rows at least.  8,190 x 4,104 bf16, codes included: 57 us, with four 56.5, sixteen
+    // 54; 32,768 x 256 f32 22.8, rows of 16 24.6; 100 x 50,000 bf16 19.3, rows of 256 20.3.
     const int64_t down = std::max<int64_t>(1, std::min<int64_t>((x.rows + 63) / 64, info.sm_count * 8 / across));
     column_amax_kernel<T, kVec><<<dim3(across, static_cast<unsigned>(down)), kAmaxThreads, 0, stream>>>(x, amax);
     return cudaGetLastError();
   }
   if (x.stride == x.cols) x = {x.data, 1, x.rows * x.cols, x.rows * x.cols, x.type};
+  // Four vectors a thread, 32 CTAs an SM at most.  8,192 x 8,192 f32 in strided rows, codes included: 102 us, with one
+  // vector 121, eight CTAs 107; 8,190 x 4,104 bf16 45.5 us, 16 vectors 47.9, eight CTAs 47.3.
   const unsigned across = ceil_div(std::max<int64_t>(x.cols / P, 1), kAmaxThreads * 4);
   const unsigned most = static_cast<unsigned>(info.sm_count) * 32;
   const dim3 grid(std::min(across, most), static_cast<unsigned>(std::min<int64_t>(x.rows, std::max(1u, most / across))));

@@ -413,7 +413,7 @@ join_kernel(const uint2* __restrict__ sorted, int64_t n, int tile, float scale, 
     last += stop ? __ffs(stop) - 1 : 32;
     if (stop) break;
   }
-  const bool shared = last - j >= 128;
+  const bool shared = last - j >= 128;  // (32,768 x 2,048 bf16, 7 in 10 tokens alike: 85 us, from 32 on 85, from 512 on 94)
   auto sum_of = [&](int64_t c, int64_t first, int step) {
     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 16
@@ -462,7 +462,10 @@ join_kernel(const uint2* __restrict__ sorted, int64_t n, int tile, float scale, 
 
 int64_t partial_pitch(int64_t cols) { return (cols + 7) / 8 * 8; }
 
-// Long tiles leave fewer partials; short ones fill the GPU: up to eight CTAs on each of 148 SMs.
+// Long tiles leave fewer partials; short ones fill the GPU: up to eight CTAs on each of a B200's 148 SMs (the size of
+// the workspace is asked for without a device).  32,768 x 2,048 bf16, 7 in 10 tokens alike: 85 us, with four CTAs an SM
+// 87, sixteen 137, tiles of 32 at most 129; 65,536 x 1,024, all alike: 90, 84, 144 and 128.  At least 8 tokens:
+// 1,999 x 1,024 f32 28.6 us, at least 4 or 16 29.3.
 int64_t tile_of(int64_t n, int64_t slices) {
   return std::max<int64_t>(8, std::min<int64_t>(kTileMost, (n * slices + 148 * 8 - 1) / (148 * 8)));
 }
@@ -528,6 +531,8 @@ cudaError_t gradient(const void* tokens, int token_bytes, const Dense& grad, flo
   kernel<<<static_cast<unsigned>(tiles * slices), kSegmentThreads, 0, stream>>>(sorted, n, tile, grad, scale, out, partials,
                                                                                 static_cast<int>(slices));
   if ((err = cudaGetLastError()) != cudaSuccess || tiles == 1) return err;
+  // A CTA per 1,024 columns, and four at least: 32,768 x 2,048 bf16 58.6 us, 85 where 7 in 10 tokens are alike.  One per
+  // 128 columns 67.9 and 72.6: more CTAs that find nothing to join; one per 1,024 throughout 57.7 and 111.
   const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(std::min<int64_t>(16, std::max((out.cols + 1023) / 1024, std::min<int64_t>(4, (out.cols + 255) / 256)))));
   join_kernel<O><<<grid, 32 * kJoinWarps, 0, stream>>>(sorted, n, tile, scale, out, partials);
   return cudaGetLastError();
