@@ -17,11 +17,12 @@ _NONE = (None, 0)
 
 
 def _row_values(value: float | torch.Tensor, name: str, rows: int, device: torch.device) -> _RowValues:
-    if not isinstance(value, torch.Tensor):
+    if value.__class__ is float or not isinstance(value, torch.Tensor):
         return _RowValues(None, 0, float(value))
-    if value.dtype != torch.float32 or value.device != device or tuple(value.shape) not in ((), (1,), (rows,)):
+    shape = value.shape
+    if value.dtype is not torch.float32 or value.device != device or shape not in ((), (1,), (rows,)):
         raise ValueError(f"{name} must be a number or a float32 tensor with one value per row")
-    return _RowValues(value.data_ptr(), value.stride(0) if value.dim() == 1 and value.shape[0] > 1 else 0, 1.0)
+    return _RowValues(value.data_ptr(), value.stride(0) if shape and shape[0] > 1 else 0, 1.0)
 
 
 def _lengths(value: torch.Tensor, name: str, rows: int, device: torch.device) -> int:

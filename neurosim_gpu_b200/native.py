@@ -362,9 +362,10 @@ def refuse_gradients(message: str, *values) -> None:
     """Raise where one of the values requires a gradient or has a tangent, which the call would drop."""
     if torch.is_grad_enabled():
         for value in values:
-            if getattr(value, "requires_grad", False):
+            if value is not None and value.__class__ is not float and getattr(value, "requires_grad", False):
                 raise ValueError(message)
-    refuse_tangents(message, *values)
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        refuse_tangents(message, *values)
 
 
 def written(out: torch.Tensor) -> None:
