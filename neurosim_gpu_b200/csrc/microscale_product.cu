@@ -23,7 +23,7 @@
 // which are tensor copies throughout, complete on its barriers.
 //
 // Few rows are bound by reading the weights: 1 x 32,000 x 4,096 15.3 us, 4.8 TB/s.  Many are bound by the tensor
-// cores, 76 % of the time active: 8,192 x 8,192 x 4,096 109 us, 5.0 PFLOP/s; x 32,768 764 us, 5.8 PFLOP/s.
+// cores, 77 % of the time active: 8,192 x 8,192 x 4,096 104-107 us, 5.2 PFLOP/s; x 32,768 770 us, 5.7 PFLOP/s.
 //
 // Where there are too few tiles for the GPU, a cluster of 2, 4 or 8 CTAs shares a tile along K: each
 // leaves its float32 partial sums in its shared memory, and each adds a part of the columns of all
