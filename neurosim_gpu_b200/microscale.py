@@ -248,6 +248,7 @@ class _Readout(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
+        refuse_tangents("nvfp4_readout has no forward-mode derivative", grad)
         state, weight, largest = ctx.saved_tensors
         wants_state, wants_weight, wants_bias, _ = ctx.needs_input_grad
         if state.shape[0] == 0:

@@ -47,8 +47,21 @@ def test_products_refuse_gradients_that_they_would_drop():
             call()
         with torch.no_grad():
             assert bool(call().isfinite().all())
-    # Forward-over-reverse reaches neither backward pass.
     with forward_ad.dual_level():
         dual = forward_ad.make_dual(x.detach(), torch.ones_like(x))
         with pytest.raises(ValueError, match="forward-mode"):
             nvfp4_readout(dual, torch.randn(6, 64, device="cuda", requires_grad=True))
+
+
+@pytest.mark.gpu
+def test_backward_passes_refuse_tangents():
+    """Forward over reverse: the gradient that comes in is a dual tensor."""
+    leaf = torch.randn(6, 64, device="cuda", requires_grad=True)
+    tokens = torch.tensor([1, 5, 1], device="cuda")
+    for y in (nvfp4_readout(torch.randn(3, 64, device="cuda"), leaf), stimulus_drive(tokens, leaf)):
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y))
+            with pytest.raises(ValueError, match="forward-mode|gradients"):
+                torch.autograd.grad(y, leaf, dual, retain_graph=True)
+        (grad,) = torch.autograd.grad(y, leaf, torch.ones_like(y))
+        assert bool(grad.any())
